@@ -17,6 +17,7 @@
 #define TI_STATUS_TMA_WAIT 1     // a wait for a TMA load ran out
 #define TI_STATUS_MMA_WAIT 2     // a wait for tensor-core work ran out
 #define TI_STATUS_PIPE_WAIT 3    // a wait for a pipeline slot ran out
+#define TI_STATUS_BEAMS 4        // a beam's parent, slot or page is not one that the call allows (nothing was moved for it)
 
 // Device address of the library's status word (one per device), for kernels to report to.
 int* ti_status_ptr();

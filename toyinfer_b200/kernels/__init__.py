@@ -554,7 +554,7 @@ def uniform_from(seed: int, key: int, step: int) -> float:
 
 
 _STATUS = {1: "a wait for a TMA load ran out", 2: "a wait for tensor-core work ran out",
-           3: "a wait for a pipeline slot ran out"}
+           3: "a wait for a pipeline slot ran out", 4: "a beam's parent, slot or page was out of place (nothing was moved for it)"}
 
 
 def reset_scratch() -> None:

@@ -1,0 +1,196 @@
+"""Beam search's kernels: the selection over beams and vocabulary (csrc/beam_select.cu), page tables and moves from the
+sequences' lengths and the beams' parents (csrc/beam_tables.cu), and the move of pages and states (csrc/beam_reorder.cu).
+
+A *group* is one request's beams; a beam's *place* is its index in the group, and belongs to one slot of the cache.  After
+``select`` the sequence at a place goes on from its parent's; ``tables`` and ``reorder`` let the cache follow, on the device:
+nothing of a step has to pass through the host before the next one starts.
+
+    choice = select(logits, scores, beams, stop_ids)
+    moves = tables(slots, choice.parents, lengths, extra, [Table(...), ...])
+    reorder(areas, moves)
+"""
+from __future__ import annotations
+
+import ctypes
+from ctypes import c_int, c_longlong, c_void_p
+from typing import NamedTuple, Optional, Sequence
+
+import torch
+
+from . import KernelError, _call, _need_cuda, _ptr, _stream
+from .lib import declare
+from .wide import _fn
+from ..cache.allocators import PAGE
+
+P, I, L = c_void_p, c_int, c_longlong
+BEAMS_MAX = 32          # beams of one group
+STOPS_MAX = 16          # stop tokens
+TABLES_MAX = 8          # page tables of one cache
+MOVES_MAX = 8192        # entries of one call's moves, over its lists
+PIECE = 8192            # bytes that a warp moves at a time (csrc/beam_reorder.cu)
+
+
+_scratch_bytes = None
+
+
+def _here(*tensors, what: str) -> None:
+    """All on the current device: the launch goes to its stream."""
+    _need_cuda(*tensors, what=what)
+    now = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != now:
+            raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{now}")
+
+
+class Choice(NamedTuple):
+    """What ``select`` gives, [groups, beams] each.  By place: the next beams' scores (-inf: no beam), the places they come from (a
+    place itself, or one whose parent is itself) and their tokens.  By rank: the candidates that ended, each at the rank it had among
+    all candidates (-inf, -1 and -1 elsewhere)."""
+
+    scores: torch.Tensor
+    parents: torch.Tensor
+    tokens: torch.Tensor
+    ended_scores: torch.Tensor
+    ended_parents: torch.Tensor
+    ended_tokens: torch.Tensor
+
+
+def select(logits: torch.Tensor, scores: torch.Tensor, beams: int, stop_ids: Optional[torch.Tensor] = None, ending: bool = True) -> Choice:
+    """The next ``beams`` beams of every group.  logits float32 [groups * held, vocab] (a group's rows follow one another), scores
+    float32 [groups, held] with held <= beams: the logarithms of the beams' probabilities so far (-inf: no beam; its row is not read).
+
+    A continuation's total is its beam's score plus log softmax of its row; larger totals come first, then lower (beam, token).  The
+    first ``beams`` whose token is not in ``stop_ids`` (int32, at most 16) are the next beams; with ``ending`` those among the first
+    ``beams`` of all whose token is in it are returned as ended.  NaN counts as -inf, +inf as the largest finite number, and what is
+    at -inf is never chosen: a group with fewer continuations keeps places without a beam.  The first child of a beam stays at its
+    place, the other children take the places of beams without one, in order.  Totals are formed in 64 bits and returned in 32."""
+    global _scratch_bytes
+    _here(logits, scores, stop_ids, what="beam select")
+    if logits.dtype != torch.float32 or logits.dim() != 2 or logits.stride(1) != 1:
+        raise KernelError("beam select: expected float32 [rows, vocab] with dense rows")
+    if scores.dtype != torch.float32 or scores.dim() != 2 or not scores.is_contiguous():
+        raise KernelError("beam select: scores must be dense float32 [groups, beams]")
+    G, held = scores.shape
+    R, V = logits.shape
+    if R != G * held or R == 0 or V == 0:
+        raise KernelError(f"beam select: {R} rows of {V} logits do not fit {G} groups of {held} beams")
+    if not 1 <= held <= beams <= BEAMS_MAX:
+        raise KernelError(f"beam select: {beams} beams from {held} (at most {BEAMS_MAX}, and no fewer than before)")
+    n_stops = 0
+    if stop_ids is not None:
+        if stop_ids.dtype != torch.int32 or stop_ids.dim() != 1 or not stop_ids.is_contiguous():
+            raise KernelError("beam select: stop tokens must be dense int32")
+        n_stops = stop_ids.numel()
+        if n_stops > STOPS_MAX:
+            raise KernelError(f"beam select: {n_stops} stop tokens (at most {STOPS_MAX})")
+    if _scratch_bytes is None:
+        _scratch_bytes = declare("ti_beam_select_scratch_bytes", [I, I, I, I], c_longlong)
+    scratch = torch.empty(_scratch_bytes(R, V, beams, n_stops), dtype=torch.uint8, device=logits.device)
+    f = torch.empty((2, G, beams), dtype=torch.float32, device=logits.device)
+    i = torch.empty((4, G, beams), dtype=torch.int32, device=logits.device)
+    out = Choice(f[0], i[0], i[1], f[1], i[2], i[3])
+    _call(_fn("ti_beam_select", [P, L, I, I, I, P, I, P, I, I, P, P, P, P, P, P, P, P]),
+          _ptr(logits), logits.stride(0), G, held, V, _ptr(scores), beams, _ptr(stop_ids), n_stops, 1 if ending else 0,
+          *(_ptr(t) for t in out), _ptr(scratch), _stream(), launches=2)
+    return out
+
+
+class Table(NamedTuple):
+    """A cache group's page table as ``tables`` changes it, int32 [slots + 1, columns] on the device; ``home``: the same with the pages
+    that each slot was given by the cache; ``ring_rows``: positions that a windowed group's ring holds (0: all positions are kept)."""
+
+    table: torch.Tensor
+    home: torch.Tensor
+    ring_rows: int = 0
+
+
+def tables(slots: torch.Tensor, parents: torch.Tensor, lengths: torch.Tensor, extra: int, page_tables: Sequence[Table]) -> torch.Tensor:
+    """Lets the page tables follow the beams, in place, and returns what has to move: int32 [1 + tables, groups * beams, 3] with
+    (source, destination, rows) per place, rows 0 where nothing does.  List 0 is slots (for states), list 1 + i pages of table i.
+
+    slots and parents int32 [groups, beams], parents as ``select`` gives them; lengths int32 [groups]: the positions that each
+    group's sequences hold are lengths + extra.  A page that is not written any more is shared by the places that come from its
+    beam; at the column that the next token goes to every place gets a page of its own, out of the group's homes there, and the
+    rows that it holds so far are among the moves.  At that column the homes of a group are pages of its own, one per place."""
+    _here(slots, parents, lengths, *(t for pt in page_tables for t in pt[:2]), what="beam tables")
+    for t, what in ((slots, "slots"), (parents, "parents"), (lengths, "lengths")):
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            raise KernelError(f"beam tables: {what} must be dense int32")
+    if slots.dim() != 2 or parents.shape != slots.shape or lengths.shape != slots.shape[:1] or slots.numel() == 0:
+        raise KernelError("beam tables: expected slots and parents [groups, beams] and lengths [groups]")
+    G, B = slots.shape
+    if B > BEAMS_MAX or len(page_tables) > TABLES_MAX:
+        raise KernelError(f"beam tables: {B} beams, {len(page_tables)} tables (at most {BEAMS_MAX} and {TABLES_MAX})")
+    words = (c_longlong * (4 * max(1, len(page_tables))))()
+    n_slots = None
+    for i, (table, home, ring_rows) in enumerate(page_tables):
+        if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous() or home.dtype != torch.int32 \
+                or home.shape != table.shape or not home.is_contiguous():
+            raise KernelError("beam tables: a table and its homes must be dense int32 [slots + 1, columns] of one shape")
+        if ring_rows < 0 or ring_rows % PAGE or (n_slots is not None and table.shape[0] != n_slots):
+            raise KernelError(f"beam tables: a ring of {ring_rows} rows, {table.shape[0]} slots")
+        n_slots = table.shape[0]
+        words[4 * i:4 * i + 4] = [table.data_ptr(), home.data_ptr(), table.shape[1], ring_rows // PAGE]
+    moves = torch.empty((1 + len(page_tables), G * B, 3), dtype=torch.int32, device=slots.device)
+    _call(_fn("ti_beam_tables", [P, I, P, P, P, I, I, I, I, I, P, P]), words, len(page_tables), _ptr(slots), _ptr(parents), _ptr(lengths),
+          int(extra), G, B, PAGE, n_slots if n_slots is not None else 1 << 30, _ptr(moves), _stream(),
+          launches=max(1, -(-len(page_tables) // 4)))
+    return moves
+
+
+class Areas:
+    """Where ``reorder`` finds a cache's memory; made once.  ``states``: tensors [slots, ...]; ``pages``: per table, in the order that
+    ``tables`` gets them, its tensors [layers, pages, kv heads, PAGE, dim].  All dense, on one device; the tensors are kept alive."""
+
+    FIELDS = 12
+
+    def __init__(self, states: Sequence[torch.Tensor], pages: Sequence[Sequence[torch.Tensor]]):
+        if len(pages) > TABLES_MAX:
+            raise KernelError(f"beam areas: {len(pages)} page tables (at most {TABLES_MAX})")
+        self.tensors = [list(states)] + [list(of_table) for of_table in pages]
+        every = [t for tensors in self.tensors for t in tensors]
+        _need_cuda(*every, what="beam areas")
+        self.device = every[0].device if every else None
+        records, self.first, self.pieces = [], [0], []
+        for which, tensors in enumerate(self.tensors):
+            before = 0
+            for t in tensors:
+                if not t.is_contiguous() or t.device != self.device or t.dim() < (1 if which == 0 else 5) or t.numel() == 0:
+                    raise KernelError(f"beam areas: {tuple(t.shape)} is not a dense tensor of "
+                                      f"{'states [slots, ...]' if which == 0 else 'pages [layers, pages, heads, rows, dim]'} on {self.device}")
+                e = t.element_size()
+                if which == 0:
+                    row = t.stride(0) * e
+                    n_outer, outer, n_inner, inner, unit, units, rows = 1, 0, 1, 0, row, t.shape[0], 1
+                else:
+                    if t.dim() != 5 or t.shape[3] != PAGE:
+                        raise KernelError(f"beam areas: pages {tuple(t.shape)} are not [layers, pages, heads, {PAGE}, dim]")
+                    n_outer, units, n_inner, rows, _ = t.shape
+                    outer, unit, inner, row = t.stride(0) * e, t.stride(1) * e, t.stride(2) * e, t.stride(3) * e
+                width = next((w for w in (16, 4, 2) if not any(x % w for x in (t.data_ptr(), outer, inner, unit, row))), 0)
+                if width == 0 or units >= 1 << 31:
+                    raise KernelError(f"beam areas: {tuple(t.shape)} of {t.dtype} cannot be moved (elements of 2 or 4 bytes)")
+                per_run = -(-(rows * row) // PIECE)
+                records.append([t.data_ptr(), outer, n_outer, inner, n_inner, unit, units, row, rows, width, per_run, before])
+                before += n_outer * n_inner * per_run
+            self.first.append(len(records))
+            self.pieces.append(before)
+        self.n_areas = len(records)
+        self.records = torch.tensor(records, dtype=torch.int64, device=self.device) if records else None
+        self._first = (c_int * len(self.first))(*self.first)
+        self._pieces = (c_longlong * len(self.pieces))(*self.pieces)
+
+
+def reorder(areas: Areas, moves: torch.Tensor) -> None:
+    """Copies what ``moves`` (from ``tables``) names: states from slot to slot, and of every layer's pages the first rows from page
+    to page.  No move may read what another one writes (``tables`` sees to that)."""
+    lists = len(areas.tensors)
+    if moves.dtype != torch.int32 or moves.dim() != 3 or moves.shape[0] != lists or moves.shape[2] != 3 or not moves.is_contiguous():
+        raise KernelError(f"beam reorder: moves must be dense int32 [{lists}, places, 3]")
+    if moves.shape[1] == 0 or moves.shape[0] * moves.shape[1] > MOVES_MAX:
+        raise KernelError(f"beam reorder: {moves.shape[0]} lists of {moves.shape[1]} moves (at most {MOVES_MAX} in all)")
+    if areas.n_areas == 0:
+        return
+    _here(moves, areas.records, what="beam reorder")
+    _call(_fn("ti_beam_reorder", [P, I, I, P, P, P, I, P]), _ptr(areas.records), areas.n_areas, lists, ctypes.cast(areas._first, P),
+          ctypes.cast(areas._pieces, P), _ptr(moves), moves.shape[1], _stream())
