@@ -110,33 +110,21 @@ def move(states, pages, moves):
 def search(logits_of, prompt, beams, max_new, stops=(), length_penalty=1.0, early_stopping=False, max_len=None):
     """The whole search without a cache: ``logits_of(tokens)`` gives the logits after them.  Returns [(value, score, tokens, reason)],
     best first, at most ``beams``: value = score / number of drawn tokens (a stop token counts) ** length_penalty."""
-    live = [(0.0, [])]
-    done = []
-
-    def value(score, n):
-        return score / n ** length_penalty
-
-    for step in range(1, max_new + 1):
+    limit = max_new if max_len is None else min(max_new, max_len - len(prompt))
+    live, done = [(0.0, [])], []
+    for step in range(1, limit + 1):
         cand = []
         for b, (score, toks) in enumerate(live):
-            lp = log_probs(logits_of(list(prompt) + toks))
-            total = score + lp
-            for t in np.argsort(-total, kind="stable")[:beams + len(stops)]:
-                cand.append((-total[t], b, int(t)))
+            total = score + log_probs(logits_of(list(prompt) + toks))
+            cand += [(-total[t], b, int(t)) for t in np.argsort(-total, kind="stable")[:beams + len(stops)] if total[t] > -np.inf]
         cand.sort()
-        for c in cand[:beams]:
-            if c[2] in stops:
-                done.append((value(-c[0], step), -c[0], live[c[1]][1], "stop"))
+        done += [(-c[0] / step ** length_penalty, -c[0], live[c[1]][1], "stop") for c in cand[:beams] if c[2] in stops]
         done = sorted(done, key=lambda d: -d[0])[:beams]
         live = [(-c[0], live[c[1]][1] + [c[2]]) for c in [c for c in cand if c[2] not in stops][:beams]]
-        if len(done) == beams:
-            best = max(s for s, _ in live)
-            # a score only falls; its value is best at the greatest length that it can reach when longer is better
-            reach = max(value(best, step + 1), value(best, max_new)) if step < max_new else -math.inf
-            if early_stopping or reach <= done[-1][0]:
-                return done
-        if max_len is not None and len(prompt) + step >= max_len:
-            break
-    reason = "context" if max_len is not None and len(prompt) + len(live[0][1]) >= max_len and len(live[0][1]) < max_new else "length"
-    done += [(value(s, len(t)), s, t, reason) for s, t in live]
+        if not live:
+            return done
+        # a score only falls, and its value is best at the greatest length that it can reach
+        if len(done) == beams and step < limit and (early_stopping or max(s for s, _ in live) / limit ** length_penalty <= done[-1][0]):
+            return done
+    done += [(s / limit ** length_penalty, s, t, "length" if limit == max_new else "context") for s, t in live]
     return sorted(done, key=lambda d: -d[0])[:beams]

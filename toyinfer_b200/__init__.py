@@ -8,8 +8,8 @@ cache with slots (cache/), one step function, a generation loop and entry points
 kernels/).
 """
 from . import models  # noqa: F401  (registers the architectures)
-from .engine import LLM, Engine, GenerationResult
-from .sampling import GREEDY, SamplingParams
+from .engine import LLM, Engine, GenerationResult, Hypothesis
+from .sampling import GREEDY, BeamParams, SamplingParams
 
-__all__ = ["LLM", "Engine", "GenerationResult", "GREEDY", "SamplingParams"]
+__all__ = ["LLM", "Engine", "GenerationResult", "Hypothesis", "GREEDY", "BeamParams", "SamplingParams"]
 __version__ = "0.1.0"

@@ -21,6 +21,11 @@ serves as key and value at once).  An entry whose mixer is several mixers side b
 with a tuple of requests and gets a tuple of views in the same order (keys and values for
 one of them, a state for another); each member is placed as an entry's single request would be.
 
+The beams of one request share pages (``reserve_beams``, ``follow_parents``): the first slot holds the prompt, the others
+bring pages of their own from the prompt's last column on, and from then on the device rewrites the group's rows of the
+page tables after every selection (kernels/beam.py).  The host's copy of those rows stays what each slot was given
+(its pages go back with the slot, wherever the group's sequences used them), and is kept on the device beside the table.
+
 The reference keeps one sequence's keys and values as [layers, max_seq_len, kv_dim]
 (src/transformer.cpp:188-195) and the position in a host variable
 (src/engine_runtime.cpp:441).
@@ -81,23 +86,30 @@ class _KVGroup:
         self.table_host = np.zeros((n_slots + 1, self.pages_per_seq), dtype=np.int32)
         self.table = torch.zeros((n_slots + 1, self.pages_per_seq), dtype=torch.int32, device=device)
         self.slot_pages: Dict[int, List[int]] = {}
+        self.slot_first: Dict[int, int] = {}           # the column of a slot's first own page, where it is not 0
         self.dirty: Dict[int, Tuple[int, int]] = {}
+        self.home: Optional[torch.Tensor] = None       # [slots + 1, pages_per_seq]: the pages that the slots of beams were given
+        self.on_device: set = set()                    # slots whose rows the device rewrites
 
     def pages_needed(self, length: int) -> int:
         n = pages_for(length)
         return min(n, self.ring_pages) if self.ring_pages else n
 
-    def grow(self, slot: int, length: int) -> None:
+    def grow(self, slot: int, length: int, first: int = 0) -> None:
+        """Pages up to ``length`` positions; ``first``: the column at which a slot without pages begins."""
         have = self.slot_pages.setdefault(slot, [])
+        if first and not have:
+            self.slot_first[slot] = first
+        held = self.slot_first.get(slot, 0) + len(have)
         need = self.pages_needed(length)
         if need > self.pages_per_seq:
             raise CacheError(
                 f"a sequence of {length} positions needs {need} pages; the cache was sized for "
                 f"{self.pages_per_seq} per sequence"
             )
-        if need > len(have):
-            new = self.pool.allocate(need - len(have))
-            a = len(have)
+        if need > held:
+            new = self.pool.allocate(need - held)
+            a = held
             have.extend(new)
             self.table_host[slot, a:need] = new
             lo, hi = self.dirty.get(slot, (a, need))
@@ -107,19 +119,37 @@ class _KVGroup:
         pages = self.slot_pages.pop(slot, [])
         self.pool.release(pages)
         self.table_host[slot, :] = 0
+        self.slot_first.pop(slot, None)
+        self.on_device.discard(slot)
         self.dirty.pop(slot, None)
 
     def flush(self) -> None:
         if not self.dirty:
             return
         first, last = min(self.dirty), max(self.dirty)
-        if len(self.dirty) > 1 and (last + 1 - first) * self.pages_per_seq <= 8192:
+        if len(self.dirty) > 1 and (last + 1 - first) * self.pages_per_seq <= 8192 and not any(first <= s <= last for s in self.on_device):
             # one copy of the rows from the first to the last (those between them are the same on both sides, or nobody's)
             self.table[first:last + 1].copy_(torch.from_numpy(self.table_host[first:last + 1]))
         else:
             for slot, (lo, hi) in self.dirty.items():
                 self.table[slot, lo:hi].copy_(torch.from_numpy(self.table_host[slot, lo:hi]))
         self.dirty.clear()
+
+    def beam_columns(self, prompt: int, length: int) -> int:
+        """The column from which every beam of a request brings pages of its own: the first that its beams write (a ring that
+        wraps comes back to all of them)."""
+        return 0 if self.ring_pages and length > self.ring_rows else min(prompt // PAGE, self.pages_needed(length))
+
+    def begin_beams(self, slots: Sequence[int]) -> None:
+        """The rows of ``slots`` are the device's from now on."""
+        self.flush()
+        if self.home is None:
+            self.home = torch.zeros_like(self.table)
+        rows = torch.from_numpy(self.table_host[list(slots)]).to(self.table.device)
+        at = torch.tensor(list(slots), dtype=torch.long, device=self.table.device)
+        self.home[at] = rows
+        self.table[at] = rows              # (whole rows: the columns of the prompt hold nothing of an earlier sequence either)
+        self.on_device.update(slots)
 
     def view(self, entry: int) -> KVView:
         i = self.entries.index(entry)
@@ -177,6 +207,7 @@ class CacheManager:
         for req, entries in by_key.items():
             self.kv_groups.append(_KVGroup(req, entries, self.n_slots, self.max_tokens,
                                            self.max_seq_len, dtype, device))
+        self._areas = None                             # the move of beams' memory: made at the first search
         self._views: Dict[int, Any] = {}
         for g in self.kv_groups:
             for e in g.entries:
@@ -202,6 +233,44 @@ class CacheManager:
             raise CacheError(f"a sequence of {new_length} positions exceeds the limit of {self.max_seq_len}")
         for g in self.kv_groups:
             g.grow(slot, new_length)
+
+    # -- beams ------------------------------------------------------------------
+    def beam_tokens(self, prompt: int, length: int, beams: int) -> int:
+        """Positions, in whole pages, that a request's beams may come to hold: the most of any group."""
+        most = 0
+        for g in self.kv_groups:
+            pages = g.pages_needed(length)
+            most = max(most, pages + (beams - 1) * (pages - g.beam_columns(prompt, length)))
+        return most * PAGE if self.kv_groups else beams * pages_for(length) * PAGE
+
+    def reserve_beams(self, slots: Sequence[int], prompt: int, length: int) -> None:
+        """Pages for the beams of one request, up to ``length`` positions each: ``slots[0]`` will run the prompt, of
+        ``prompt`` tokens, the others share its pages and bring their own from the first that they write."""
+        if length > self.max_seq_len:
+            raise CacheError(f"a sequence of {length} positions exceeds the limit of {self.max_seq_len}")
+        for s in slots:
+            if not self.slots.is_live(s):
+                raise CacheError(f"slot {s} is not in use")
+        for g in self.kv_groups:
+            first = g.beam_columns(prompt, length)
+            g.grow(slots[0], length)
+            for s in slots[1:]:
+                g.grow(s, length, first)
+            g.begin_beams(slots)
+
+    def begin_beams(self, slots: Sequence[int], prompt: int) -> None:
+        """The prompt has run in ``slots[0]``: the other slots count as holding it too (``follow_parents`` comes next)."""
+        for s in slots[1:]:
+            self.length[s] = prompt
+
+    def follow_parents(self, slots: torch.Tensor, parents: torch.Tensor, lengths: torch.Tensor, extra: int) -> None:
+        """Lets every place of the groups ``slots`` [groups, beams] go on from the place ``parents`` names (kernels/beam.py:
+        tables, reorder); the sequences hold ``lengths`` [groups] + extra positions.  All on the device, in the stream's order."""
+        from ..kernels import beam as KB
+        if self._areas is None:
+            self._areas = KB.Areas(list(self.states.values()), [[g.k] if g.v is None else [g.k, g.v] for g in self.kv_groups])
+        moves = KB.tables(slots, parents, lengths, extra, [KB.Table(g.table, g.home, g.ring_rows) for g in self.kv_groups])
+        KB.reorder(self._areas, moves)
 
     def commit(self, slot: int, new_length: int) -> None:
         self.length[slot] = new_length

@@ -46,8 +46,9 @@ __device__ __forceinline__ void copy_piece(char* dst, const char* src, int bytes
     for (; i < n; i += 32) d[i] = s[i];
 }
 
+// It lets no later kernel start before it ends: attention kernels read page tables and earlier rows before they wait for the kernel
+// before them, as no other kernel writes those.
 __global__ void __launch_bounds__(RT) beam_reorder_kernel(ReorderArgs a) {
-    ti_pdl_trigger();
     extern __shared__ int active[];          // [lists, n_moves]: the moves that copy something
     __shared__ int count[LISTS_MAX];
     ti_pdl_sync();

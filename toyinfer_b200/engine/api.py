@@ -3,6 +3,7 @@ in, generated token ids out.
 
     llm = LLM("path/to/model", dtype="bfloat16", max_seq_len=8192)
     results = llm.generate([[1, 2, 3], [4, 5]], SamplingParams(temperature=0.0), max_new_tokens=16)
+    best = llm.beam_search([[1, 2, 3], [4, 5]], BeamParams(beams=4), max_new_tokens=16)
 
 Prompts are token ids: the reference's tokenizer and chat template
 (src/tokenizer.cpp) are not part of this library.  Option names follow the
@@ -14,7 +15,8 @@ from typing import List, Optional, Sequence
 
 import torch
 
-from ..sampling import GREEDY, Sampler, SamplingParams
+from ..sampling import GREEDY, BeamParams, Sampler, SamplingParams
+from .beam import BeamLoop, BeamStepper, Hypothesis
 from .engine import Engine, parse_dtype
 from .generate import GenerationLoop, GenerationResult, GenerationStats
 
@@ -154,4 +156,24 @@ class LLM:
         if e.device.type == "cuda":
             from .. import kernels as K
             K.check_status()     # raises if a kernel gave up on a bounded wait: its tokens are not to be trusted
+        return out
+
+    def beam_search(self, prompts: Sequence[Sequence[int]], beams: Optional[BeamParams] = None, max_new_tokens: int = 16,
+                    stop_token_ids: Optional[Sequence[int]] = None, ignore_eos: bool = False) -> List[List[Hypothesis]]:
+        """The ``beams.n_best`` best hypotheses of every prompt, best first.  Each request takes ``beams.beams`` of the engine's
+        ``max_batch`` places; the beams share the pages of their prompt."""
+        beams = beams or BeamParams()
+        beams.check()
+        stops = set()
+        if not ignore_eos:
+            stops.update(self.stop_token_ids)
+            stops.update(int(t) for t in stop_token_ids or ())
+        e = self.engine
+        loop = BeamLoop(BeamStepper(e, beams, sorted(stops)), beams, sorted(stops), e.max_batch, e.max_seq_len, e.cache.max_tokens,
+                        dedicated_prefill=self.use_dedicated_prefill, prefill_chunk=self.prefill_chunk)
+        out = loop.run(prompts, max_new_tokens)
+        self.last_stats = loop.stats
+        if e.device.type == "cuda":
+            from .. import kernels as K
+            K.check_status()
         return out

@@ -1,9 +1,8 @@
 """Command line, with the reference's option names and meanings where it has them
 (src/options.cpp:7-45): --model_dir, --max_seq_len, --use_dedicated_prefill,
 --use_multi_stream, --enable_cuda_graph, --detail_time, --bench, --temperature, --top_k,
---top_p.  Prompts are token ids, not text: the reference's tokenizer, chat template
-(--thinking) and terminal REPL are not part of this library, and neither is its beam
-search (--beam_size above 1 is refused).
+--top_p, --beam_size, --length_penalty.  Prompts are token ids, not text: the reference's
+tokenizer, chat template (--thinking) and terminal REPL are not part of this library.
 
     bin/toyinfer --model_dir DIR --max_seq_len 4096 --prompt_ids "1,2,3;4,5" --max_new_tokens 32
     bin/toyinfer --model_dir DIR --max_seq_len 8192 --bench long
@@ -64,8 +63,9 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--temperature", type=float, default=0.6)
     ap.add_argument("--top_k", type=int, default=20)
     ap.add_argument("--top_p", type=float, default=0.95)
-    ap.add_argument("--beam_size", type=int, default=1, help="only 1 (no beam search)")
-    ap.add_argument("--length_penalty", type=float, default=1.0, help="unused without beam search")
+    ap.add_argument("--beam_size", type=int, default=1, help="beams per request (1: no beam search); with more, the best "
+                    "hypothesis is printed and the sampling options have no effect")
+    ap.add_argument("--length_penalty", type=float, default=1.0, help="beam search ranks hypotheses by score / tokens ** length_penalty")
     # beyond the reference
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
     ap.add_argument("--prompt_ids", default="", help='token ids: "1,2,3;4,5" or a file')
@@ -110,8 +110,14 @@ def detail_lines(st, report, cuda_graph: bool) -> List[str]:
 
 def main(argv=None) -> int:
     args = build_parser().parse_args(argv)
-    if args.beam_size != 1:
-        print("toyinfer: beam search is not part of this library (--beam_size must be 1)", file=sys.stderr)
+    from ..sampling import BeamParams
+    beams = BeamParams(beams=args.beam_size, length_penalty=args.length_penalty)
+    try:
+        beams.check()
+        if args.beam_size > args.max_batch:
+            raise ValueError(f"--beam_size {args.beam_size} exceeds --max_batch {args.max_batch}")
+    except ValueError as exc:
+        print(f"toyinfer: {exc}", file=sys.stderr)
         return 2
     if bool(args.model_dir) == bool(args.random):
         print("toyinfer: give either --model_dir or --random CONFIG_JSON", file=sys.stderr)
@@ -142,10 +148,14 @@ def main(argv=None) -> int:
         prompts = _prompts(args.prompt_ids)
     params = SamplingParams(temperature=args.temperature, top_k=args.top_k, top_p=args.top_p, seed=args.seed)
     t0 = time.perf_counter()
-    results = llm.generate(prompts, params, max_new_tokens=max_new, ignore_eos=ignore_eos)
+    if args.beam_size > 1:
+        results = [hyps[0] for hyps in llm.beam_search(prompts, beams, max_new_tokens=max_new, ignore_eos=ignore_eos)]
+    else:
+        results = llm.generate(prompts, params, max_new_tokens=max_new, ignore_eos=ignore_eos)
     wall = time.perf_counter() - t0
     for i, r in enumerate(results):
-        print(json.dumps({"request": i, "tokens": r.tokens, "finish_reason": r.finish_reason}))
+        line = {"request": i, "tokens": r.tokens, "finish_reason": r.finish_reason}
+        print(json.dumps(line if args.beam_size == 1 else {**line, "score": r.score}))
     st = llm.last_stats
     total = st.prompt_tokens + st.generated_tokens
     print(f"[perf] prompt_tokens={st.prompt_tokens} generated_tokens={st.generated_tokens} "

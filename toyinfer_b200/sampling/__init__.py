@@ -1,5 +1,5 @@
 """Sampling options and the sampler."""
-from .params import GREEDY, SamplingParams
+from .params import GREEDY, BeamParams, SamplingParams
 from .sampler import Sampler
 
-__all__ = ["GREEDY", "SamplingParams", "Sampler"]
+__all__ = ["GREEDY", "BeamParams", "SamplingParams", "Sampler"]
