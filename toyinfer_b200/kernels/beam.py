@@ -85,14 +85,14 @@ def select(logits: torch.Tensor, scores: torch.Tensor, beams: int, stop_ids: Opt
             raise KernelError(f"beam select: {n_stops} stop tokens (at most {STOPS_MAX})")
     if _scratch_bytes is None:
         _scratch_bytes = declare("ti_beam_select_scratch_bytes", [I, I, I, I], c_longlong)
-    scratch = torch.empty(_scratch_bytes(R, V, beams, n_stops), dtype=torch.uint8, device=logits.device)
     f = torch.empty((2, G, beams), dtype=torch.float32, device=logits.device)
     i = torch.empty((4, G, beams), dtype=torch.int32, device=logits.device)
-    out = Choice(f[0], i[0], i[1], f[1], i[2], i[3])
-    _call(_fn("ti_beam_select", [P, L, I, I, I, P, I, P, I, I, P, P, P, P, P, P, P, P]),
-          _ptr(logits), logits.stride(0), G, held, V, _ptr(scores), beams, _ptr(stop_ids), n_stops, 1 if ending else 0,
-          *(_ptr(t) for t in out), _ptr(scratch), _stream(), launches=2)
-    return out
+    scratch = torch.empty(_scratch_bytes(R, V, beams, n_stops), dtype=torch.uint8, device=logits.device)
+    _call(_fn("ti_beam_select", [P, L, I, I, I, P, I, P, I, I, P, P, P, P]),
+          logits.data_ptr(), logits.stride(0), G, held, V, scores.data_ptr(), beams, _ptr(stop_ids), n_stops, 1 if ending else 0,
+          f.data_ptr(), i.data_ptr(), scratch.data_ptr(), _stream(), launches=2)
+    (scores, ended_scores), (parents, tokens, ended_parents, ended_tokens) = f.unbind(0), i.unbind(0)
+    return Choice(scores, parents, tokens, ended_scores, ended_parents, ended_tokens)
 
 
 class Table(NamedTuple):
