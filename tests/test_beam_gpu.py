@@ -53,8 +53,16 @@ def test_select_sizes(G, held, B, V, n_stops, pad):
     check_select(x, s, B, stops, ending=False)
 
 
+@pytest.mark.parametrize("held,B,V", [(1, 8, 5000), (1, 32, 20001), (1, 32, 3000), (2, 30, 40000), (1, 24, 1024 * 23), (3, 32, 152000), (32, 32, 152000)])
+def test_select_with_fewer_tiles_than_beams(held, B, V):
+    x, s = inputs(2, held, V, seed=V, pad=B % 3)
+    s[1, 1:] = -float("inf")                     # one beam left
+    x[0, 5] = 15.0
+    check_select(x, s, B, [5, 17])
+
+
 @pytest.mark.parametrize("kind", ["equal", "coarse", "rising", "falling", "one thread", "lowest", "few allowed", "peaked", "tiny range", "far apart"])
-@pytest.mark.parametrize("V", [50, 3000, 20000])
+@pytest.mark.parametrize("V", [50, 3000, 20000, 200000])
 def test_select_values(kind, V):
     G, B = 3, 6
     x, s = inputs(G, B, V, seed=5)

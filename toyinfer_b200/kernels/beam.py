@@ -11,14 +11,12 @@ nothing of a step has to pass through the host before the next one starts.
 """
 from __future__ import annotations
 
-import ctypes
 from ctypes import c_int, c_longlong, c_void_p
 from typing import NamedTuple, Optional, Sequence
 
 import torch
 
-from . import KernelError, _call, _need_cuda, _ptr, _stream
-from .lib import declare
+from . import KernelError, _call, _need_cuda, _ptr, _raw_device, _stream
 from .wide import _fn
 from ..cache.allocators import PAGE
 
@@ -27,18 +25,16 @@ BEAMS_MAX = 32          # beams of one group
 STOPS_MAX = 16          # stop tokens
 TABLES_MAX = 8          # page tables of one cache
 MOVES_MAX = 8192        # entries of one call's moves, over its lists
+TILE, PART = 1024, 4    # logits of a row that csrc/beam_select.cu takes at a time, and the words of scratch for them
 PIECE = 8192            # bytes that a warp moves at a time (csrc/beam_reorder.cu)
-
-
-_scratch_bytes = None
 
 
 def _here(*tensors, what: str) -> None:
     """All on the current device: the launch goes to its stream."""
-    _need_cuda(*tensors, what=what)
-    now = torch.cuda.current_device()
+    now = _raw_device() if _raw_device is not None else torch.cuda.current_device()
     for t in tensors:
-        if t is not None and t.device.index != now:
+        if t is not None and t.get_device() != now:          # (-1: not a CUDA device)
+            _need_cuda(t, what=what)
             raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{now}")
 
 
@@ -64,7 +60,6 @@ def select(logits: torch.Tensor, scores: torch.Tensor, beams: int, stop_ids: Opt
     ``beams`` of all whose token is in it are returned as ended.  NaN counts as -inf, +inf as the largest finite number, and what is
     at -inf is never chosen: a group with fewer continuations keeps places without a beam.  The first child of a beam stays at its
     place, the other children take the places of beams without one, in order.  Totals are formed in 64 bits and returned in 32."""
-    global _scratch_bytes
     _here(logits, scores, stop_ids, what="beam select")
     if logits.dtype != torch.float32 or logits.dim() != 2 or logits.stride(1) != 1:
         raise KernelError("beam select: expected float32 [rows, vocab] with dense rows")
@@ -83,16 +78,16 @@ def select(logits: torch.Tensor, scores: torch.Tensor, beams: int, stop_ids: Opt
         n_stops = stop_ids.numel()
         if n_stops > STOPS_MAX:
             raise KernelError(f"beam select: {n_stops} stop tokens (at most {STOPS_MAX})")
-    if _scratch_bytes is None:
-        _scratch_bytes = declare("ti_beam_select_scratch_bytes", [I, I, I, I], c_longlong)
-    f = torch.empty((2, G, beams), dtype=torch.float32, device=logits.device)
-    i = torch.empty((4, G, beams), dtype=torch.int32, device=logits.device)
-    scratch = torch.empty(_scratch_bytes(R, V, beams, n_stops), dtype=torch.uint8, device=logits.device)
+    # results and scratch in one piece: each allocation takes the host as long as half a launch
+    n = G * beams
+    at = (6 * n + 3) & ~3
+    room = torch.empty(at + R * (-(-V // TILE)) * PART, dtype=torch.int32, device=logits.device)
+    base = room.data_ptr()
     _call(_fn("ti_beam_select", [P, L, I, I, I, P, I, P, I, I, P, P, P, P]),
           logits.data_ptr(), logits.stride(0), G, held, V, scores.data_ptr(), beams, _ptr(stop_ids), n_stops, 1 if ending else 0,
-          f.data_ptr(), i.data_ptr(), scratch.data_ptr(), _stream(), launches=2)
-    (scores, ended_scores), (parents, tokens, ended_parents, ended_tokens) = f.unbind(0), i.unbind(0)
-    return Choice(scores, parents, tokens, ended_scores, ended_parents, ended_tokens)
+          base, base + 8 * n, base + 4 * at, _stream(), launches=2)
+    scores, ended_scores, parents, tokens, ended_parents, ended_tokens = room[:6 * n].view(6, G, beams).unbind(0)
+    return Choice(scores.view(torch.float32), parents, tokens, ended_scores.view(torch.float32), ended_parents, ended_tokens)
 
 
 class Table(NamedTuple):
@@ -121,16 +116,18 @@ def tables(slots: torch.Tensor, parents: torch.Tensor, lengths: torch.Tensor, ex
     G, B = slots.shape
     if B > BEAMS_MAX or len(page_tables) > TABLES_MAX:
         raise KernelError(f"beam tables: {B} beams, {len(page_tables)} tables (at most {BEAMS_MAX} and {TABLES_MAX})")
-    words = (c_longlong * (4 * max(1, len(page_tables))))()
+    words = []
     n_slots = None
-    for i, (table, home, ring_rows) in enumerate(page_tables):
-        if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous() or home.dtype != torch.int32 \
-                or home.shape != table.shape or not home.is_contiguous():
+    for table, home, ring_rows in page_tables:
+        shape = table.shape
+        if table.dtype != torch.int32 or len(shape) != 2 or not table.is_contiguous() or home.dtype != torch.int32 \
+                or home.shape != shape or not home.is_contiguous():
             raise KernelError("beam tables: a table and its homes must be dense int32 [slots + 1, columns] of one shape")
-        if ring_rows < 0 or ring_rows % PAGE or (n_slots is not None and table.shape[0] != n_slots):
-            raise KernelError(f"beam tables: a ring of {ring_rows} rows, {table.shape[0]} slots")
-        n_slots = table.shape[0]
-        words[4 * i:4 * i + 4] = [table.data_ptr(), home.data_ptr(), table.shape[1], ring_rows // PAGE]
+        if ring_rows < 0 or ring_rows % PAGE or (n_slots is not None and shape[0] != n_slots):
+            raise KernelError(f"beam tables: a ring of {ring_rows} rows, {shape[0]} slots")
+        n_slots = shape[0]
+        words += (table.data_ptr(), home.data_ptr(), shape[1], ring_rows // PAGE)
+    words = (c_longlong * len(words))(*words)
     moves = torch.empty((1 + len(page_tables), G * B, 3), dtype=torch.int32, device=slots.device)
     _call(_fn("ti_beam_tables", [P, I, P, P, P, I, I, I, I, I, P, P]), words, len(page_tables), _ptr(slots), _ptr(parents), _ptr(lengths),
           int(extra), G, B, PAGE, n_slots if n_slots is not None else 1 << 30, _ptr(moves), _stream(),
@@ -184,13 +181,13 @@ class Areas:
 def reorder(areas: Areas, moves: torch.Tensor) -> None:
     """Copies what ``moves`` (from ``tables``) names: states from slot to slot, and of every layer's pages the first rows from page
     to page.  No move may read what another one writes (``tables`` sees to that)."""
-    lists = len(areas.tensors)
-    if moves.dtype != torch.int32 or moves.dim() != 3 or moves.shape[0] != lists or moves.shape[2] != 3 or not moves.is_contiguous():
+    lists, shape = len(areas.tensors), moves.shape
+    if moves.dtype != torch.int32 or len(shape) != 3 or shape[0] != lists or shape[2] != 3 or not moves.is_contiguous():
         raise KernelError(f"beam reorder: moves must be dense int32 [{lists}, places, 3]")
-    if moves.shape[1] == 0 or moves.shape[0] * moves.shape[1] > MOVES_MAX:
-        raise KernelError(f"beam reorder: {moves.shape[0]} lists of {moves.shape[1]} moves (at most {MOVES_MAX} in all)")
+    if shape[1] == 0 or lists * shape[1] > MOVES_MAX:
+        raise KernelError(f"beam reorder: {lists} lists of {shape[1]} moves (at most {MOVES_MAX} in all)")
     if areas.n_areas == 0:
         return
     _here(moves, areas.records, what="beam reorder")
-    _call(_fn("ti_beam_reorder", [P, I, I, P, P, P, I, P]), _ptr(areas.records), areas.n_areas, lists, ctypes.cast(areas._first, P),
-          ctypes.cast(areas._pieces, P), _ptr(moves), moves.shape[1], _stream())
+    _call(_fn("ti_beam_reorder", [P, I, I, P, P, P, I, P]), _ptr(areas.records), areas.n_areas, lists, areas._first, areas._pieces,
+          moves.data_ptr(), shape[1], _stream())
