@@ -26,12 +26,12 @@ constexpr int BEAMS_MAX = 32;        // a group's beams: one bit of a warp's wor
 constexpr int STOPS_MAX = 16;
 constexpr int TILE = 1024;           // logits that a warp takes
 constexpr int LANE = TILE / 32;
-constexpr int MT = 256;              // threads of a merge block
+constexpr int MT = 512;              // threads of a merge block
 constexpr int MW = MT / 32;
 constexpr int TILES = 512;           // tiles of a group that may reach the bound
 constexpr int ROOM = 1536;           // candidates above it; more than a tile and all that is kept of the ones before
-constexpr int KEYS = 4096;           // tiles of a group whose totals are kept in shared memory
-constexpr int AHEAD = 4;             // tiles on the way at a time, when they are read again
+constexpr int KEYS = 3840;           // tiles of a group whose totals are kept in shared memory
+constexpr int AHEAD = 4;             // pairs of tiles on the way at a time, when they are read again
 constexpr int HELD = 5;              // tiles of a row, of 32 each, whose parts a warp has on the way at a time
 constexpr float BIG = 3.402823466e38f;
 constexpr float PLAIN = 600.f;       // |largest logit| of a tile up to which its exponentials are summed as they are
@@ -239,33 +239,38 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
         for (int s = 0; s < a.n_stops; ++s) stop |= stops[s] == token;
         return stop;
     };
-    // each row's sum, by a warp; the tiles' top logits into shared memory
+    // A tile whose top logit is a stop token's says nothing about the others' totals.
+#pragma unroll 1
+    for (int i = MT - 1 - tid; i < a.held * a.n_stops; i += MT) {
+        const int b = i / a.n_stops, id = stops[i % a.n_stops], at = b * a.tiles + id / TILE;
+        if (id < 0 || id >= a.V || at >= KEYS) continue;
+        const float w = logits[(size_t)b * a.ld + id], top = part[at].top;
+        if (fminf(w, BIG) == top) atomicOr(&stop_tile[at >> 5], 1u << (at & 31));
+    }
+    // Each row's sum, by a warp, and from it the keys of its tiles' largest totals: 0 where a tile has no candidate.
 #pragma unroll 1
     for (int b = warp; b < a.held; b += MW) {
         const Part* p = part + (size_t)b * a.tiles;
         const float score = scores[b];
         float m = -INFINITY, lowest = INFINITY;
         double sum = 0.0;
+        Part q[HELD];
 #pragma unroll 1
         for (int t0 = 0; t0 < a.tiles; t0 += HELD * 32) {
-            Part q[HELD];
 #pragma unroll
             for (int j = 0; j < HELD; ++j) q[j] = t0 + j * 32 + lane < a.tiles ? p[t0 + j * 32 + lane] : Part{0.0, -INFINITY, 0.f};
 #pragma unroll
-            for (int j = 0; j < HELD; ++j) {
-                const int i = b * a.tiles + t0 + j * 32 + lane;
-                if (t0 + j * 32 + lane < a.tiles && i < KEYS) tile_key[i] = __float_as_uint(q[j].top);
+            for (int j = 0; j < HELD; ++j)
                 if (q[j].top > -INFINITY) {
                     m = fmaxf(m, q[j].ref);
                     lowest = fminf(lowest, q[j].ref);
                     sum += q[j].sum;
                 }
-            }
         }
         m = warp_max(m);
         lowest = -warp_max(-lowest);
-        if (!(score > -INFINITY) || m == -INFINITY) continue;      // (nothing was written for a row without a beam)
-        if (lowest < m) {                          // tiles that were taken against another reference
+        const bool there = score > -INFINITY && m > -INFINITY;      // (nothing was written for a row without a beam)
+        if (there && lowest < m) {                 // tiles that were taken against another reference
             sum = 0.0;
 #pragma unroll 1
             for (int t = lane; t < a.tiles; t += 32)
@@ -273,33 +278,37 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
         }
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        const double add = there ? (double)score - log(sum) : -INFINITY, ref = m;
         if (lane == 0) {
-            row_add[b] = (double)score - log(sum);
-            row_ref[b] = m;
+            row_add[b] = add;
+            row_ref[b] = ref;
+        }
+#pragma unroll 1
+        for (int t0 = 0; t0 < a.tiles; t0 += HELD * 32) {
+#pragma unroll
+            for (int j = 0; j < HELD; ++j) {
+                const int t = t0 + j * 32 + lane, i = b * a.tiles + t;
+                if (t >= a.tiles || i >= KEYS) continue;
+                const float top = a.tiles > HELD * 32 ? p[t].top : q[j].top;
+                tile_key[i] = there && top > -INFINITY ? short_key(add + ((double)top - ref)) : 0u;
+            }
         }
     }
-#pragma unroll 1
-    for (int i = tid; i < a.held * a.n_stops; i += MT) {
-        const int b = i / a.n_stops, id = stops[i % a.n_stops], t = id / TILE;
-        if (id < 0 || id >= a.V || !(scores[b] > -INFINITY)) continue;
-        const float w = fminf(logits[(size_t)b * a.ld + id], BIG);
-        if (w == part[b * a.tiles + t].top && b * a.tiles + t < KEYS) atomicOr(&stop_tile[(b * a.tiles + t) >> 5], 1u << ((b * a.tiles + t) & 31));
-    }
     __syncthreads();
-    // the key of tile i's largest total; 0 where it has no candidate.  (Tiles behind the shared ones are read again each time, and
-    // count for the bound only if no stop token is among them.)
-    auto key_of_tile = [&](int i, float top) {
+    // (Tiles behind the shared ones are read again each time, and count for the bound only where there are no stop tokens.)
+    auto key_behind = [&](int i) {
         const int b = i / a.tiles;
+        const float top = part[i].top;
         return row_add[b] > -INFINITY && top > -INFINITY ? short_key(row_add[b] + ((double)top - row_ref[b])) : 0u;
     };
     unsigned mine = KEY_NONE;
+    const int shared = min(all, KEYS);
+#pragma unroll 2
+    for (int i = tid; i < shared; i += MT)
+        if (!((stop_tile[i >> 5] >> (i & 31)) & 1u)) mine = max(mine, tile_key[i]);
+    if (a.n_stops == 0)
 #pragma unroll 1
-    for (int i = tid; i < all; i += MT) {
-        const bool shared = i < KEYS;
-        const unsigned key = key_of_tile(i, shared ? __uint_as_float(tile_key[i]) : part[i].top);
-        if (shared) tile_key[i] = key;
-        if (shared ? !((stop_tile[i >> 5] >> (i & 31)) & 1u) : a.n_stops == 0) mine = max(mine, key);
-    }
+        for (int i = KEYS + tid; i < all; i += MT) mine = max(mine, key_behind(i));
     keys[tid] = mine;
     __syncthreads();
     if (warp == 0) {
@@ -314,12 +323,16 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
     }
     __syncthreads();
     unsigned bound = s_bound;
+    auto list = [&](int i) {
+        const int to = atomicAdd(&n_tiles, 1);
+        if (to < TILES) tile_list[to] = (i / a.tiles) << 24 | (i % a.tiles);
+    };
+#pragma unroll 2
+    for (int i = tid; i < shared; i += MT)
+        if (tile_key[i] >= bound) list(i);
 #pragma unroll 1
-    for (int i = tid; i < all; i += MT)
-        if ((i < KEYS ? tile_key[i] : key_of_tile(i, part[i].top)) >= bound) {
-            const int to = atomicAdd(&n_tiles, 1);
-            if (to < TILES) tile_list[to] = (i / a.tiles) << 24 | (i % a.tiles);
-        }
+    for (int i = KEYS + tid; i < all; i += MT)
+        if (key_behind(i) >= bound) list(i);
     __syncthreads();
     // a logit's total, and whether it is a candidate at all
     auto candidate = [&](int b, float w, double& total) {
@@ -344,38 +357,42 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
     for (int attempt = 0; attempt < 2 && listed <= TILES && n > ROOM; ++attempt) {
         mine = KEY_NONE;
 #pragma unroll 1
-        for (int i0 = 0; i0 < listed; i0 += AHEAD) {
+        for (int i0 = tid >> 8; i0 < listed; i0 += 2 * AHEAD) {          // half of the block to a tile, four logits a thread
+            const int part_of = tid & 255;
             float v[AHEAD][4];
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
-                const int what = tile_list[min(i0 + u, listed - 1)];
+                const int what = tile_list[min(i0 + 2 * u, listed - 1)];
                 const float* x = logits + (size_t)(what >> 24) * a.ld;
                 const int at = (what & 0xFFFFFF) * TILE;
                 if (VEC && at + TILE <= a.V) {
-                    const float4 q = *reinterpret_cast<const float4*>(x + at + tid * 4);
+                    const float4 q = *reinterpret_cast<const float4*>(x + at + part_of * 4);
                     v[u][0] = q.x; v[u][1] = q.y; v[u][2] = q.z; v[u][3] = q.w;
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const int c = at + (VEC ? tid * 4 + e : e * MT + tid);
+                        const int c = at + (VEC ? part_of * 4 + e : e * 256 + part_of);
                         v[u][e] = c < a.V ? x[c] : -INFINITY;
                     }
                 }
             }
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
-                const int what = tile_list[min(i0 + u, listed - 1)], b = what >> 24, at = (what & 0xFFFFFF) * TILE;
+                const int what = tile_list[min(i0 + 2 * u, listed - 1)], b = what >> 24, at = (what & 0xFFFFFF) * TILE;
                 const float cut = row_cut[b];
-                if (i0 + u >= listed || !(fmaxf(fmaxf(v[u][0], v[u][1]), fmaxf(v[u][2], v[u][3])) >= cut)) continue;
-                float w[4] = {v[u][0], v[u][1], v[u][2], v[u][3]};
-#pragma unroll 1
-                for (int e = 0; e < 4; ++e) {
+                if (i0 + 2 * u >= listed) continue;
+                unsigned hits = 0u;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) hits |= v[u][e] >= cut ? 1u << e : 0u;          // (a NaN is none)
+                while (hits) {
+                    const int e = __ffs(hits) - 1;
+                    const float w = e < 2 ? (e ? v[u][1] : v[u][0]) : (e == 2 ? v[u][2] : v[u][3]);
+                    hits &= hits - 1u;
                     double total;
-                    if (candidate(b, w[0], total)) {
+                    if (candidate(b, w, total)) {
                         const unsigned key = short_key(total);
-                        if (key >= bound && !take(total, b, at + (VEC ? tid * 4 + e : e * MT + tid))) mine = max(mine, key);
+                        if (key >= bound && !take(total, b, at + (VEC ? part_of * 4 + e : e * 256 + part_of))) mine = max(mine, key);
                     }
-                    w[0] = w[1]; w[1] = w[2]; w[2] = w[3];
                 }
             }
         }
@@ -458,9 +475,7 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
         __syncthreads();
         n = n_found;
     }
-    for (int i = tid; i < n; i += MT) {
-        int rank, open;
-        rank_of(i, rank, open);
+    auto place_of_rank = [&](int i, int rank, int open) {
         const unsigned long long whose = found_at[i];
         const float total = (float)total_of(found_key[i]);
         if (whose < STOP) {
@@ -473,6 +488,29 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
             a.end_score[o + rank] = total;
             a.end_parent[o + rank] = (int)((whose & ~STOP) >> 32);
             a.end_token[o + rank] = (int)whose;
+        }
+    };
+    if (n <= 256) {
+        // a warp to an entry, a lane to one it is compared with
+#pragma unroll 1
+        for (int i = warp; i < n; i += MW) {
+            const unsigned long long key = found_key[i], at = found_at[i] & ~STOP;
+            int rank = 0, open = 0;
+#pragma unroll 1
+            for (int j = lane; j - lane < n; j += 32) {
+                const unsigned long long k2 = j < n ? found_key[j] : 0ull, w2 = j < n ? found_at[j] : ~0ull;
+                const bool before = (k2 > key) | ((k2 == key) & ((w2 & ~STOP) < at));
+                rank += __popc(__ballot_sync(0xffffffffu, before));
+                open += __popc(__ballot_sync(0xffffffffu, before & (w2 < STOP)));
+            }
+            if (lane == 0) place_of_rank(i, rank, open);
+        }
+    } else {
+#pragma unroll 1
+        for (int i = tid; i < n; i += MT) {
+            int rank, open;
+            rank_of(i, rank, open);
+            place_of_rank(i, rank, open);
         }
     }
     __syncthreads();
