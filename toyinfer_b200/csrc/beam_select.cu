@@ -146,25 +146,26 @@ __global__ void __launch_bounds__(256, 4) beam_scan_kernel(ScanArgs a) {
 }
 
 // A value at or below the k-th largest (k <= 32) of the block's keys (one per thread, in shared memory), with few keys more above it
-// than k; by one warp.  Every lane holds MW of the keys, so at least 32 lie at or above the least of the lanes' largest ones: there
-// the bisection begins, and it is mostly done after a step or two.
+// than k; by one warp.  Of two keys the larger one stands for both, and every lane holds MW / 2 of those; at least 32 lie at or above
+// the least of the lanes' largest ones: there the bisection begins, and it is mostly done after a step or two.
 __device__ __forceinline__ unsigned bound_of(const unsigned* __restrict__ keys, int k) {
     const int lane = threadIdx.x & 31;
-    unsigned mine[MW], first = 0u;
+    unsigned mine[MW / 2], first = 0u;
 #pragma unroll
-    for (int i = 0; i < MW; ++i) {
-        mine[i] = keys[i * 32 + lane];
+    for (int i = 0; i < MW / 2; ++i) {
+        mine[i] = max(keys[i * 32 + lane], keys[(i + MW / 2) * 32 + lane]);
         first = max(first, mine[i]);
     }
     unsigned lo = __reduce_min_sync(0xffffffffu, first), hi = __reduce_max_sync(0xffffffffu, first);
-    const int enough = k + (k >> 2) + 1;
+    const int enough = k + (k >> 1) + 2;
     auto above = [&](unsigned bound) {
         int n = 0;
 #pragma unroll
-        for (int i = 0; i < MW; ++i) n += mine[i] >= bound;
+        for (int i = 0; i < MW / 2; ++i) n += mine[i] >= bound;
         return __reduce_add_sync(0xffffffffu, n);
     };
     if (above(max(lo, KEY_NONE + 1)) <= enough) return lo;
+#pragma unroll 1
     while (lo < hi) {
         const unsigned mid = lo + ((hi - lo) >> 1) + 1;
         const int n = above(mid);
@@ -252,7 +253,7 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
     for (int b = warp; b < a.held; b += MW) {
         const Part* p = part + (size_t)b * a.tiles;
         const float score = scores[b];
-        float m = -INFINITY, lowest = INFINITY;
+        bool some = false, shifted = false;
         double sum = 0.0;
         Part q[HELD];
 #pragma unroll 1
@@ -262,15 +263,20 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
 #pragma unroll
             for (int j = 0; j < HELD; ++j)
                 if (q[j].top > -INFINITY) {
-                    m = fmaxf(m, q[j].ref);
-                    lowest = fminf(lowest, q[j].ref);
+                    some = true;
+                    shifted |= q[j].ref != 0.f;
                     sum += q[j].sum;
                 }
         }
-        m = warp_max(m);
-        lowest = -warp_max(-lowest);
-        const bool there = score > -INFINITY && m > -INFINITY;      // (nothing was written for a row without a beam)
-        if (there && lowest < m) {                 // tiles that were taken against another reference
+        const bool there = score > -INFINITY && __any_sync(0xffffffffu, some);      // (nothing was written for a row without a beam)
+        float m = 0.f;
+        if (there && __any_sync(0xffffffffu, shifted)) {
+            // tiles that were taken against another reference than 0: all against the largest of them
+            m = -INFINITY;
+#pragma unroll 1
+            for (int t = lane; t < a.tiles; t += 32)
+                if (p[t].top > -INFINITY) m = fmaxf(m, p[t].ref);
+            m = warp_max(m);
             sum = 0.0;
 #pragma unroll 1
             for (int t = lane; t < a.tiles; t += 32)
@@ -311,18 +317,18 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
         for (int i = KEYS + tid; i < all; i += MT) mine = max(mine, key_behind(i));
     keys[tid] = mine;
     __syncthreads();
-    if (warp == 0) {
-        const unsigned b = bound_of(keys, a.beams);
-        if (lane == 0) s_bound = b;
-        // ... and below which logit a row's entries cannot reach it: a little lower, for the roundings of the two forms
+    // the bound, and below which logit a row's entries cannot reach it: a little lower, for the roundings of the two forms
+    auto cut_rows = [&](unsigned b) {
         const unsigned u = (b & 0x80000000u) ? b & 0x7FFFFFFFu : ~b;
+        if (lane == 0) s_bound = b;
         if (lane < a.held) {
             const double t = (double)__uint_as_float(u), add = row_add[lane], ref = row_ref[lane];
             row_cut[lane] = b <= KEY_NONE ? -INFINITY : __double2float_rd(((t - add) + ref) - 1e-14 * (fabs(t) + fabs(add) + fabs(ref)));
         }
-    }
+    };
+    if (warp == 0) cut_rows(bound_of(keys, a.beams));
     __syncthreads();
-    unsigned bound = s_bound;
+    const unsigned bound = s_bound;
     auto list = [&](int i) {
         const int to = atomicAdd(&n_tiles, 1);
         if (to < TILES) tile_list[to] = (i / a.tiles) << 24 | (i % a.tiles);
@@ -340,22 +346,13 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
         total = row_add[b] + ((double)fminf(w, BIG) - row_ref[b]);
         return total > -INFINITY;
     };
-    auto take = [&](double total, int b, int token) {
-        const int to = atomicAdd(&n_found, 1);
-        const bool stop = is_stop(token);
-        if (to < ROOM) {
-            found_key[to] = order_key(total);
-            found_at[to] = ((unsigned long long)b << 32 | (unsigned)token) | (stop ? STOP : 0ull);
-        }
-        return stop;
+    auto put = [&](int i, double total, int b, int token) {
+        found_key[i] = order_key(total);
+        found_at[i] = ((unsigned long long)b << 32 | (unsigned)token) | (is_stop(token) ? STOP : 0ull);
     };
+    // f(beam, token, logit) for the listed tiles' entries that reach their row's cut
     const int listed = n_tiles;
-    int n = ROOM + 1;
-    // (With fewer tiles than beams there is no bound yet, and everything may lie above it: the threads' own maxima over what they
-    // see then give one.)
-#pragma unroll 1
-    for (int attempt = 0; attempt < 2 && listed <= TILES && n > ROOM; ++attempt) {
-        mine = KEY_NONE;
+    auto each = [&](auto&& f) {
 #pragma unroll 1
         for (int i0 = tid >> 8; i0 < listed; i0 += 2 * AHEAD) {          // half of the block to a tile, four logits a thread
             const int part_of = tid & 255;
@@ -378,9 +375,9 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
             }
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
-                const int what = tile_list[min(i0 + 2 * u, listed - 1)], b = what >> 24, at = (what & 0xFFFFFF) * TILE;
-                const float cut = row_cut[b];
                 if (i0 + 2 * u >= listed) continue;
+                const int what = tile_list[i0 + 2 * u], b = what >> 24, at = (what & 0xFFFFFF) * TILE;
+                const float cut = row_cut[b];
                 unsigned hits = 0u;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) hits |= v[u][e] >= cut ? 1u << e : 0u;          // (a NaN is none)
@@ -388,25 +385,50 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
                     const int e = __ffs(hits) - 1;
                     const float w = e < 2 ? (e ? v[u][1] : v[u][0]) : (e == 2 ? v[u][2] : v[u][3]);
                     hits &= hits - 1u;
-                    double total;
-                    if (candidate(b, w, total)) {
-                        const unsigned key = short_key(total);
-                        if (key >= bound && !take(total, b, at + (VEC ? part_of * 4 + e : e * 256 + part_of))) mine = max(mine, key);
-                    }
+                    f(b, at + (VEC ? part_of * 4 + e : e * 256 + part_of), w);
                 }
             }
         }
+    };
+    auto gather = [&](int b, int token, float w) {
+        const int to = atomicAdd(&n_found, 1);
+        if (to < ROOM) {
+            found_key[to] = __float_as_uint(w);
+            found_at[to] = (unsigned long long)b << 32 | (unsigned)token;
+        }
+    };
+    int n = ROOM + 1;
+    if (listed <= TILES) {
+        each(gather);
         __syncthreads();
         n = n_found;
-        if (n <= ROOM || attempt) break;
-        keys[tid] = mine;
-        __syncthreads();
-        if (warp == 0) {
-            const unsigned b = bound_of(keys, a.beams);
-            if (lane == 0) { s_bound = b; n_found = 0; }
+        if (n > ROOM) {
+            // With fewer tiles than beams there was no bound, and everything lay above it: the threads' largest entries give one.
+            mine = KEY_NONE;
+            each([&](int b, int token, float w) {
+                double total;
+                if (candidate(b, w, total) && short_key(total) > mine && !is_stop(token)) mine = short_key(total);
+            });
+            keys[tid] = mine;
+            __syncthreads();
+            if (tid == 0) n_found = 0;
+            if (warp == 0) cut_rows(bound_of(keys, a.beams));
+            __syncthreads();
+            each(gather);
+            __syncthreads();
+            n = n_found;
+        }
+    }
+    if (n <= ROOM) {
+#pragma unroll 1
+        for (int i = tid; i < n; i += MT) {
+            const int b = (int)(found_at[i] >> 32);
+            double total;
+            // (one that is no candidate, a NaN's neighbour at -infinity: behind all others, and told apart below)
+            if (candidate(b, __uint_as_float((unsigned)found_key[i]), total)) put(i, total, b, (int)found_at[i]);
+            else found_key[i] = 0ull;
         }
         __syncthreads();
-        bound = s_bound;
     }
     // ranks of entry i among all that were found, and among those that are no stop tokens
     auto rank_of = [&](int i, int& rank, int& open) {
@@ -447,7 +469,7 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
                 const unsigned long long last = s_last;
                 for (int c = at + tid; c < min(at + TILE, a.V); c += MT) {
                     double total;
-                    if (candidate(b, logits[(size_t)b * a.ld + c], total) && order_key(total) > last) take(total, b, c);
+                    if (candidate(b, logits[(size_t)b * a.ld + c], total) && order_key(total) > last) put(atomicAdd(&n_found, 1), total, b, c);
                 }
                 __syncthreads();
                 n = n_found;             // at most a tile and two times BEAMS_MAX
@@ -477,6 +499,7 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
     }
     auto place_of_rank = [&](int i, int rank, int open) {
         const unsigned long long whose = found_at[i];
+        if (found_key[i] == 0ull) return;        // none
         const float total = (float)total_of(found_key[i]);
         if (whose < STOP) {
             if (open < a.beams) {
