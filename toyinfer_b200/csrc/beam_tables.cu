@@ -14,8 +14,8 @@
 // leaves each surviving beam at its place, so no move reads what another one writes; parents that are not so are reported in the
 // status word and left out.
 //
-// A block per group.  Everything here is a few KB: what counts is the launch, so all tables of a cache take one.  A column is read
-// and written by one thread, beams first, so the table is changed in place.
+// A block per group and table.  Everything here is a few KB: what counts is the launch and the chain of loads behind it (parents,
+// then rows, then the pages of column w), so all tables of a cache take one launch and a row is copied by a warp.
 #include "tma.cuh"
 
 namespace {
@@ -42,92 +42,81 @@ struct TablesArgs {
 
 __global__ void __launch_bounds__(TT) beam_tables_kernel(TablesArgs a) {
     ti_pdl_trigger();
-    __shared__ int slot[BEAMS_MAX], parent[BEAMS_MAX], old_at[BEAMS_MAX];
-    const int g = blockIdx.x, tid = threadIdx.x, B = a.beams;
-    ti_pdl_sync();
-    const int* slots = ti_dependent(a.slots) + (size_t)g * B;
-    const int* parents = ti_dependent(a.parents) + (size_t)g * B;
-    const int L = ti_dependent(a.lengths)[g] + a.extra;
-    if (tid < 32) {
-        int p = tid < B ? parents[tid] : tid;
-        const int s = tid < B ? slots[tid] : 0;
-        const int pp = __shfl_sync(0xffffffffu, p, p & 31);
-        const bool bad = tid < B && (p < 0 || p >= B || pp != p || s < 0 || s >= a.n_slots);
-        if (bad) {
-            ti_report(a.status, TI_STATUS_BEAMS);
-            p = tid;
-        }
-        const bool bad_slot = tid < B && (s < 0 || s >= a.n_slots);
-        slot[tid] = bad_slot ? -1 : s;
-        parent[tid] = p;
-        __syncwarp();
-        if (tid < B && slot[parent[tid]] < 0) parent[tid] = tid;
-    }
-    __syncthreads();
+    __shared__ int slot[BEAMS_MAX], parent[BEAMS_MAX], moved[BEAMS_MAX], here[BEAMS_MAX];
+    __shared__ int s_moved;
+    const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 31, B = a.beams;
     const size_t at = (size_t)g * B;
-    if (a.first == 0 && tid < B) {
-        const int p = parent[tid];
-        int* m = a.moves + (at + tid) * 3;
-        const bool goes = p != tid;
-        m[0] = goes ? slot[p] : 0;
-        m[1] = goes ? slot[tid] : 0;
-        m[2] = goes ? 1 : 0;
-    }
-    for (int k = 0; k < a.n_tables; ++k) {
-        const TableArg t = a.t[k];
-        int* table = ti_dependent(t.table);
-        const int* home = ti_dependent(t.home);
-        const int held = L > 0 ? (L + a.page - 1) / a.page : 0;
-        const int used = min(held, t.ring_pages ? min(t.ring_pages, t.width) : t.width);
-        const int w = t.ring_pages ? (max(L, 0) / a.page) % t.ring_pages : max(L, 0) / a.page;
-        const bool wrapped = t.ring_pages && L >= t.ring_pages * a.page;
-        const int rows = wrapped ? a.page : max(L, 0) % a.page;
-        const bool begun = w < used;                 // the column that is written next holds something
-        for (int c = tid; c < used; c += TT) {
-            if (c == w) continue;
-            int was[BEAMS_MAX];
-#pragma unroll
-            for (int b = 0; b < BEAMS_MAX; ++b)
-                if (b < B && parent[b] != b) was[b] = table[(size_t)slot[parent[b]] * t.width + c];
-#pragma unroll
-            for (int b = 0; b < BEAMS_MAX; ++b)
-                if (b < B && parent[b] != b) table[(size_t)slot[b] * t.width + c] = was[b];
+    ti_pdl_sync();
+    const int L = max(ti_dependent(a.lengths)[g] + a.extra, 0);
+    if (tid < 32) {
+        int p = lane < B ? ti_dependent(a.parents)[at + lane] : lane;
+        const int s = lane < B ? ti_dependent(a.slots)[at + lane] : 0;
+        const bool slot_ok = s >= 0 && s < a.n_slots;
+        const int pp = __shfl_sync(0xffffffffu, p, p & 31);
+        const bool source_ok = __shfl_sync(0xffffffffu, (int)slot_ok, p & 31);
+        if (lane < B && (p < 0 || p >= B || pp != p || !slot_ok || !source_ok)) {
+            ti_report(a.status, TI_STATUS_BEAMS);
+            p = lane;
         }
-        if (tid < 32) {
-            int* m = a.moves + ((size_t)(1 + a.first + k) * a.groups * B + at + tid) * 3;
-            int src = 0, dst = 0, n = 0;
-            const bool in = tid < B && begun && slot[tid] >= 0;
-            const int p = tid < B ? parent[tid] : tid;
-            int page = in ? table[(size_t)slot[p] * t.width + w] : -1 - tid;
-            const int mine = in ? home[(size_t)slot[tid] * t.width + w] : -1 - tid;
-            // survivors keep their page, the lowest place of those that share one
-            const unsigned stays = __ballot_sync(0xffffffffu, in && p == tid);
-            const unsigned same = __match_any_sync(0xffffffffu, page);
-            const bool keeps = in && p == tid && (__ffs(same & stays) - 1) == tid;
-            const unsigned kept = __ballot_sync(0xffffffffu, keeps);
-            old_at[tid] = page;
-            __syncwarp();
-            bool free = in;
-            for (int b = 0; b < B; ++b)
-                if (((kept >> b) & 1u) && old_at[b] == mine) free = false;
-            const unsigned offers = __ballot_sync(0xffffffffu, free);
-            const unsigned needs = __ballot_sync(0xffffffffu, in && !keeps);
-            const int turn = __popc(needs & ((1u << tid) - 1u));
-            const unsigned from = __fns(offers, 0, turn + 1);
-            const int given = __shfl_sync(0xffffffffu, mine, from < 32 ? (int)from : tid);
-            __syncwarp();
-            if (in && !keeps) {
-                if (from < 32) {
-                    table[(size_t)slot[tid] * t.width + w] = given;
-                    if (rows > 0) { src = page; dst = given; n = rows; }
-                } else {
-                    ti_report(a.status, TI_STATUS_BEAMS);       // the homes do not hold a page per beam
-                }
-            }
-            if (tid < B) { m[0] = src; m[1] = dst; m[2] = n; }
+        slot[lane] = slot_ok ? s : -1;
+        parent[lane] = p;
+        const unsigned goes = __ballot_sync(0xffffffffu, p != lane);
+        if (p != lane) moved[__popc(goes & ((1u << lane) - 1u))] = lane;
+        if (lane == 0) s_moved = __popc(goes);
+        __syncwarp();
+        if (blockIdx.y == 0 && a.first == 0 && lane < B) {
+            int* m = a.moves + (at + lane) * 3;
+            m[0] = p != lane ? slot[p] : 0;
+            m[1] = p != lane ? s : 0;
+            m[2] = p != lane ? 1 : 0;
         }
-        __syncthreads();
     }
+    if (a.n_tables == 0) return;
+    __syncthreads();
+    const TableArg t = a.t[blockIdx.y];
+    int* table = ti_dependent(t.table);
+    const int pages = L / a.page;
+    const int used = min((L + a.page - 1) / a.page, t.ring_pages ? min(t.ring_pages, t.width) : t.width);
+    const int w = t.ring_pages ? pages % t.ring_pages : pages;
+    const int rows = t.ring_pages && pages >= t.ring_pages ? a.page : L - pages * a.page;
+    // A survivor's row stays as it is at every column but w, and only survivors' rows are read: no order matters.
+    for (int j = tid >> 5; j < s_moved; j += TT / 32) {
+        const int* from = table + (size_t)slot[parent[moved[j]]] * t.width;
+        int* to = table + (size_t)slot[moved[j]] * t.width;
+#pragma unroll 4
+        for (int c = lane; c < used; c += 32)
+            if (c != w) to[c] = from[c];
+    }
+    if (tid >= 32) return;
+    int* m = a.moves + ((size_t)(1 + a.first + blockIdx.y) * a.groups * B + at + lane) * 3;
+    const bool in = lane < B && w < used && slot[lane] >= 0;         // the column that is written next holds something
+    const int p = parent[lane];
+    const int page = in ? table[(size_t)slot[p] * t.width + w] : -1 - lane;
+    const int mine = in ? ti_dependent(t.home)[(size_t)slot[lane] * t.width + w] : -1 - lane;
+    const unsigned below = (1u << lane) - 1u;
+    // survivors keep their page, the lowest place of those that share one
+    const unsigned stays = __ballot_sync(0xffffffffu, in && p == lane);
+    const unsigned same = __match_any_sync(0xffffffffu, page);
+    const bool keeps = in && p == lane && !(same & stays & below);
+    const unsigned kept = __ballot_sync(0xffffffffu, keeps);
+    bool free = in;
+    for (unsigned k = kept; k; k &= k - 1u)
+        if (__shfl_sync(0xffffffffu, page, __ffs(k) - 1) == mine) free = false;
+    const unsigned offers = __ballot_sync(0xffffffffu, free), needs = __ballot_sync(0xffffffffu, in && !keeps);
+    if (free) here[__popc(offers & below)] = mine;
+    __syncwarp();                                                    // (every page has been read: rows may change)
+    int src = 0, dst = 0, n = 0;
+    if (in && !keeps) {
+        const int turn = __popc(needs & below);
+        if (turn < __popc(offers)) {
+            const int given = here[turn];
+            table[(size_t)slot[lane] * t.width + w] = given;
+            if (rows > 0) { src = page; dst = given; n = rows; }
+        } else {
+            ti_report(a.status, TI_STATUS_BEAMS);                    // the homes do not hold a page per beam
+        }
+    }
+    if (lane < B) { m[0] = src; m[1] = dst; m[2] = n; }
 }
 }  // namespace
 
@@ -159,7 +148,7 @@ extern "C" int ti_beam_tables(const long long* tables, int n_tables, const int* 
         a.n_slots = n_slots;
         a.moves = moves;
         a.status = status;
-        TI_CUDA(ti_launch(beam_tables_kernel, dim3(groups), dim3(TT), 0, stream, a));
+        TI_CUDA(ti_launch(beam_tables_kernel, dim3(groups, a.n_tables ? a.n_tables : 1), dim3(TT), 0, stream, a));
     }
     return 0;
 }
