@@ -26,7 +26,7 @@ STOPS_MAX = 16          # stop tokens
 TABLES_MAX = 8          # page tables of one cache
 MOVES_MAX = 8192        # entries of one call's moves, over its lists
 TILE, PART = 1024, 4    # logits of a row that csrc/beam_select.cu takes at a time, and the words of scratch for them
-PIECE = 8192            # bytes that a warp moves at a time (csrc/beam_reorder.cu)
+PIECE = 16384           # bytes that a warp moves at a time (csrc/beam_reorder.cu)
 
 
 def _here(*tensors, what: str) -> None:
@@ -107,18 +107,21 @@ def tables(slots: torch.Tensor, parents: torch.Tensor, lengths: torch.Tensor, ex
     group's sequences hold are lengths + extra.  A page that is not written any more is shared by the places that come from its
     beam; at the column that the next token goes to every place gets a page of its own, out of the group's homes there, and the
     rows that it holds so far are among the moves.  At that column the homes of a group are pages of its own, one per place."""
-    _here(slots, parents, lengths, *(t for pt in page_tables for t in pt[:2]), what="beam tables")
+    _here(slots, parents, lengths, what="beam tables")
     for t, what in ((slots, "slots"), (parents, "parents"), (lengths, "lengths")):
         if t.dtype != torch.int32 or not t.is_contiguous():
             raise KernelError(f"beam tables: {what} must be dense int32")
-    if slots.dim() != 2 or parents.shape != slots.shape or lengths.shape != slots.shape[:1] or slots.numel() == 0:
+    shape = slots.shape
+    if len(shape) != 2 or parents.shape != shape or lengths.shape != shape[:1] or 0 in shape:
         raise KernelError("beam tables: expected slots and parents [groups, beams] and lengths [groups]")
-    G, B = slots.shape
-    if B > BEAMS_MAX or len(page_tables) > TABLES_MAX:
-        raise KernelError(f"beam tables: {B} beams, {len(page_tables)} tables (at most {BEAMS_MAX} and {TABLES_MAX})")
+    G, B = shape
+    n_tables = len(page_tables)
+    if B > BEAMS_MAX or n_tables > TABLES_MAX:
+        raise KernelError(f"beam tables: {B} beams, {n_tables} tables (at most {BEAMS_MAX} and {TABLES_MAX})")
     words = []
     n_slots = None
     for table, home, ring_rows in page_tables:
+        _here(table, home, what="beam tables")
         shape = table.shape
         if table.dtype != torch.int32 or len(shape) != 2 or not table.is_contiguous() or home.dtype != torch.int32 \
                 or home.shape != shape or not home.is_contiguous():
@@ -127,11 +130,10 @@ def tables(slots: torch.Tensor, parents: torch.Tensor, lengths: torch.Tensor, ex
             raise KernelError(f"beam tables: a ring of {ring_rows} rows, {shape[0]} slots")
         n_slots = shape[0]
         words += (table.data_ptr(), home.data_ptr(), shape[1], ring_rows // PAGE)
-    words = (c_longlong * len(words))(*words)
-    moves = torch.empty((1 + len(page_tables), G * B, 3), dtype=torch.int32, device=slots.device)
-    _call(_fn("ti_beam_tables", [P, I, P, P, P, I, I, I, I, I, P, P]), words, len(page_tables), _ptr(slots), _ptr(parents), _ptr(lengths),
-          int(extra), G, B, PAGE, n_slots if n_slots is not None else 1 << 30, _ptr(moves), _stream(),
-          launches=max(1, -(-len(page_tables) // 4)))
+    moves = torch.empty((1 + n_tables, G * B, 3), dtype=torch.int32, device=slots.device)
+    _call(_fn("ti_beam_tables", [P, I, P, P, P, I, I, I, I, I, P, P]), (c_longlong * len(words))(*words), n_tables, slots.data_ptr(),
+          parents.data_ptr(), lengths.data_ptr(), int(extra), G, B, PAGE, n_slots if n_slots is not None else 1 << 30, moves.data_ptr(),
+          _stream(), launches=max(1, -(-n_tables // 4)))
     return moves
 
 
