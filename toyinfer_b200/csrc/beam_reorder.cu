@@ -9,17 +9,17 @@
 //
 // The only work is bytes: each is read once and written once.  Warps take pieces of PIECE bytes, all pieces of all runs of all moves
 // in one numbering, so a few moves of a small cache spread over the SMs as many moves of a large one do.  Widths of 16, 4 or 2
-// bytes, as the area's addresses and strides allow; a warp has eight loads on the way before its first store.  As many blocks as fit
-// the SMs at once, and pieces as long as a head's page, keep the reads and writes of DRAM in long runs: 32 moves of part pages of 36
-// layers (261 MB read and written) take 43 us, 48 with 8 KB pieces and 8 blocks an SM queued, 73 with sixteen loads on the way; 40
-// at the copy rate.  Twelve states of 38 MB that start at any 4 bytes (911 MB) 150 us, at the copy rate 139.
+// bytes, as the area's addresses and strides allow; a warp has eight loads on the way before its first store.  Four blocks an SM, all
+// resident, and pieces as long as a head's page keep what DRAM reads and writes in long runs: 32 moves of part pages of 36 layers (261
+// MB read and written) take 43.4 us; 46.1 with pieces of 8 KB, 45.8 with five blocks, 48.5 with three, 73 with sixteen loads on the
+// way; 39.9 at the copy rate.  Twelve states of 38 MB that start at any 4 bytes (911 MB) take 152 us, 139 at the copy rate.
 #include "tma.cuh"
 
 namespace {
 constexpr int LISTS_MAX = 9;         // states, and up to eight page tables
 constexpr int RT = 256;
 constexpr int PIECE = 16384;         // a page of 64 rows of 128 elements of 16 bits
-constexpr int BLOCKS = 5;            // an SM, all at once
+constexpr int BLOCKS = 4;            // an SM, all at once
 
 struct Area {                        // as the host writes it: 64-bit words
     long long base, outer, n_outer, inner, n_inner, unit, units, row, rows, width, pieces, first;
@@ -52,7 +52,7 @@ __device__ __forceinline__ void copy_piece(char* dst, const char* src, int bytes
 
 // It lets no later kernel start before it ends: attention kernels read page tables and earlier rows before they wait for the kernel
 // before them, as no other kernel writes those.
-__global__ void __launch_bounds__(RT, BLOCKS) beam_reorder_kernel(ReorderArgs a) {
+__global__ void __launch_bounds__(RT) beam_reorder_kernel(ReorderArgs a) {
     extern __shared__ int active[];          // [lists, n_moves]: the moves that copy something
     __shared__ int count[LISTS_MAX];
     ti_pdl_sync();
