@@ -142,6 +142,47 @@ def test_select_is_the_same_every_time_and_reads_its_own_rows_only():
     assert all(torch.equal(p, q) for p, q in zip(d, e)) and not torch.equal(d.tokens, a.tokens)
 
 
+def test_select_of_odd_views():
+    """One row whose distance to the next is anything; a column of a wider tensor; a score that no logarithm has."""
+    x, s = inputs(1, 1, 5000, seed=2)
+    check_select(x[0].unsqueeze(1).t(), s, 4)                  # stride 1 along both
+    check_select(x.expand(1, -1)[:, 7:4001], s, 3)
+    wide = torch.randn(6, 9000, device=DEV)
+    check_select(wide[:, 100:8101], torch.zeros(3, 2, device=DEV), 2)
+    check_select(wide[::2, 4:4100], torch.zeros(1, 3, device=DEV), 3)
+    from toyinfer_b200.kernels import beam as KB
+    got = KB.select(wide[:2], torch.tensor([[float("inf"), 0.0]], device=DEV), 3, None)
+    assert got.scores.tolist() == [[float("inf")] * 3] and got.tokens.tolist() == [[0, 1, 2]] and got.parents.tolist() == [[0, 0, 0]]
+
+
+def test_two_selections_at_once():
+    """On two streams, and from two graphs replayed side by side: each has scratch of its own."""
+    from toyinfer_b200.kernels import beam as KB
+    made = [inputs(8, 4, 60000, seed=k) for k in (1, 2)]
+    want = [KB.select(x, s, 4, None) for x, s in made]
+    streams, graphs = [torch.cuda.Stream() for _ in made], []
+    for (x, s), st in zip(made, streams):
+        st.wait_stream(torch.cuda.current_stream())
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            graphs.append((g, KB.select(x, s, 4, None)))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for (g, _), st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    for w, (_, got) in zip(want, graphs):
+        assert all(torch.equal(a, b) for a, b in zip(w, got))
+    for _ in range(5):
+        got = []
+        for (x, s), st in zip(made, streams):
+            with torch.cuda.stream(st):
+                got.append(KB.select(x, s, 4, None))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for w, k in zip(want, got) for a, b in zip(w, k))
+
+
 # -- tables ------------------------------------------------------------------------------------------------------------
 class Made:
     """Slots, homes and tables of groups that have searched for a while, with pages shared as a search leaves them."""
@@ -232,6 +273,69 @@ def test_parents_out_of_place_are_reported_and_left_out():
         want_table = m.table.copy()
         want = plain.tables([want_table], [m.home], [0], m.slots, good, m.lengths)
         assert np.array_equal(moves.cpu().numpy(), want) and np.array_equal(table.cpu().numpy(), want_table)
+
+
+def test_slots_and_homes_out_of_place_are_reported_and_left_out():
+    from toyinfer_b200 import kernels as K
+    from toyinfer_b200.kernels import beam as KB
+    m = Made(5, 1, 3, [70], 3)
+    lengths, parents = m.dev(np.array([70], dtype=np.int32)), m.dev(np.array([[0, 0, 0]], dtype=np.int32))
+    for bad in ([m.n_slots + 1, 0, 1], [0, -1, 1], [0, 1, 1]):
+        table = m.dev(m.table)
+        moves = KB.tables(m.dev(np.array([bad], dtype=np.int32)), parents, lengths, 0, [KB.Table(table, m.dev(m.home))])
+        with pytest.raises(K.KernelError, match="out of place"):
+            K.check_status()
+        rows = [s for s in bad if 0 <= s <= m.n_slots and bad.count(s) == 1]
+        other = [s for s in range(m.n_slots + 1) if s not in rows]
+        assert np.array_equal(table.cpu().numpy()[other], m.table[other])
+        assert all(0 <= x <= m.n_slots for x in moves[0, :, :2].flatten().tolist())
+    home = m.home.copy()
+    home[m.slots[0, 1:], 1] = 0                       # slots that brought no page for the column that is written
+    table = m.dev(m.table)
+    table[torch.from_numpy(m.slots[0]).long().to(DEV), 1] = int(m.home[m.slots[0, 0], 1])
+    moves = KB.tables(m.dev(m.slots), parents, lengths, 0, [KB.Table(table, m.dev(home))])
+    with pytest.raises(K.KernelError, match="out of place"):
+        K.check_status()
+    assert moves[1].abs().sum().item() == 0
+
+
+def test_captured_and_replayed_with_other_parents():
+    """The three kernels in one graph: a replay reads the parents and lengths that are there then, and gives what plain calls give."""
+    from toyinfer_b200 import kernels as K
+    from toyinfer_b200.kernels import beam as KB
+    G, B, V = 4, 4, 3000
+    m = Made(8, G, B, [100, 64, 130, 191], 4)
+    pages = torch.randn(2, m.n_slots * 4 + 1, 2, PAGE, 16, device=DEV)
+    state = torch.randn(m.n_slots + 1, 33, device=DEV)
+    x, s = inputs(G, B, V, seed=4)
+    slots, home, lengths = m.dev(m.slots), m.dev(m.home), m.dev(np.array(m.lengths, dtype=np.int32))
+
+    def memory_of():
+        return m.dev(m.table), pages.clone(), state.clone()
+
+    def search(x, s, table, page, st, areas):
+        c = KB.select(x, s, B, None)
+        KB.reorder(areas, KB.tables(slots, c.parents, lengths, 0, [KB.Table(table, home)]))
+        return c
+
+    table, page, st = memory_of()
+    areas = KB.Areas([st], [[page]])
+    search(x, s, table, page, st, areas)              # (sets everything up)
+    table.copy_(m.dev(m.table)), page.copy_(pages), st.copy_(state)
+    xs, ss = x.clone(), s.clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = search(xs, ss, table, page, st, areas)
+    for seed in (11, 12):
+        nx, ns = inputs(G, B, V, seed=seed)
+        xs.copy_(nx), ss.copy_(ns)
+        table.copy_(m.dev(m.table)), page.copy_(pages), st.copy_(state)
+        g.replay()
+        t2, p2, s2 = memory_of()
+        want = search(nx, ns, t2, p2, s2, KB.Areas([s2], [[p2]]))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert torch.equal(table, t2) and torch.equal(page, p2) and torch.equal(st, s2) and not torch.equal(table, m.dev(m.table))
+    K.check_status()
 
 
 # -- the move ----------------------------------------------------------------------------------------------------------

@@ -49,6 +49,23 @@ def test_search_matches_plain(model_folders, graph, name, lens, beams, max_new):
         assert all_free(llm)
 
 
+@pytest.mark.parametrize("penalty,early,chunk,dedicated", [(1.0, False, None, True), (0.0, True, 20, True), (2.5, False, 7, True), (0.7, False, None, False)])
+def test_requests_that_end_at_different_steps(model_folders, penalty, early, chunk, dedicated):
+    """Many stop tokens, more requests than a batch holds, prompts in pieces or token by token: requests leave a running batch while the
+    others' next step is under way, and some meet the engine's length limit."""
+    from toyinfer_b200 import LLM, BeamParams
+    llm = LLM(model_folders["B"], dtype="float32", max_seq_len=96, max_batch=10, max_tokens=2048, prefill_chunk=chunk, use_dedicated_prefill=dedicated)
+    prompts = prompts_for("B", [20, 60, 90, 5, 64, 1, 33], seed=12)
+    stops = [11, 12] + list(range(100, 112))             # the model's own two and more
+    got = llm.beam_search(prompts, BeamParams(3, penalty, early, 3), max_new_tokens=14, stop_token_ids=stops)
+    ends = set()
+    for p, g in zip(prompts, got):
+        same(g, plain_search(model_folders["B"], p, 3, 14, stops=stops, length_penalty=penalty, early_stopping=early, max_len=96))
+        ends.add(max(len(h.tokens) for h in g))
+    assert len(ends) > 1 and any(h.finish_reason == "context" for g in got for h in g) and llm.last_stats.batches == 3
+    assert all_free(llm)
+
+
 def test_one_beam_is_greedy_and_batches_do_not_matter(model_folders):
     from toyinfer_b200 import LLM, BeamParams, SamplingParams
     llm = LLM(model_folders["B"], dtype="float32", max_seq_len=256, max_batch=8, max_tokens=4096)

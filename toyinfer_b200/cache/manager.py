@@ -140,8 +140,8 @@ class _KVGroup:
         wraps comes back to all of them)."""
         return 0 if self.ring_pages and length > self.ring_rows else min(prompt // PAGE, self.pages_needed(length))
 
-    def begin_beams(self, slots: Sequence[int]) -> None:
-        """The rows of ``slots`` are the device's from now on."""
+    def give_to_device(self, slots: Sequence[int]) -> None:
+        """The rows of ``slots`` are the device's from now on, until the slots are given back."""
         self.flush()
         if self.home is None:
             self.home = torch.zeros_like(self.table)
@@ -256,7 +256,7 @@ class CacheManager:
             g.grow(slots[0], length)
             for s in slots[1:]:
                 g.grow(s, length, first)
-            g.begin_beams(slots)
+            g.give_to_device(slots)
 
     def begin_beams(self, slots: Sequence[int], prompt: int) -> None:
         """The prompt has run in ``slots[0]``: the other slots count as holding it too (``follow_parents`` comes next)."""

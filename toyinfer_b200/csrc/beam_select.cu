@@ -323,7 +323,8 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
         if (lane == 0) s_bound = b;
         if (lane < a.held) {
             const double t = (double)__uint_as_float(u), add = row_add[lane], ref = row_ref[lane];
-            row_cut[lane] = b <= KEY_NONE ? -INFINITY : __double2float_rd(((t - add) + ref) - 1e-14 * (fabs(t) + fabs(add) + fabs(ref)));
+            const double cut = ((t - add) + ref) - 1e-14 * (fabs(t) + fabs(add) + fabs(ref));
+            row_cut[lane] = b <= KEY_NONE || cut != cut ? -INFINITY : __double2float_rd(cut);
         }
     };
     if (warp == 0) cut_rows(bound_of(keys, a.beams));

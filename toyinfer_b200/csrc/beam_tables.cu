@@ -11,8 +11,8 @@
 //     whole page where the ring has wrapped.
 //
 // A place whose parent is another place needs that place's state as well: a move (source slot, destination slot, 1).  The selection
-// leaves each surviving beam at its place, so no move reads what another one writes; parents that are not so are reported in the
-// status word and left out.
+// leaves each surviving beam at its place, so no move reads what another one writes; parents that are not so, slots outside the
+// tables or twice in a group, and homes without a page per beam are reported in the status word and left out.
 //
 // A block per group and table.  Everything here is a few KB: what counts is the launch and the chain of loads behind it (parents,
 // then rows, then the pages of column w), so all tables of a cache take one launch and a row is copied by a warp.
@@ -51,7 +51,8 @@ __global__ void __launch_bounds__(TT) beam_tables_kernel(TablesArgs a) {
     if (tid < 32) {
         int p = lane < B ? ti_dependent(a.parents)[at + lane] : lane;
         const int s = lane < B ? ti_dependent(a.slots)[at + lane] : 0;
-        const bool slot_ok = s >= 0 && s < a.n_slots;
+        const unsigned twins = __match_any_sync(0xffffffffu, lane < B ? s : -1 - lane);
+        const bool slot_ok = s >= 0 && s < a.n_slots && (twins & (twins - 1u)) == 0u;        // a slot of its own
         const int pp = __shfl_sync(0xffffffffu, p, p & 31);
         const bool source_ok = __shfl_sync(0xffffffffu, (int)slot_ok, p & 31);
         if (lane < B && (p < 0 || p >= B || pp != p || !slot_ok || !source_ok)) {
@@ -99,7 +100,7 @@ __global__ void __launch_bounds__(TT) beam_tables_kernel(TablesArgs a) {
     const unsigned same = __match_any_sync(0xffffffffu, page);
     const bool keeps = in && p == lane && !(same & stays & below);
     const unsigned kept = __ballot_sync(0xffffffffu, keeps);
-    bool free = in;
+    bool free = in && mine > 0;                                      // (page 0 is nobody's)
     for (unsigned k = kept; k; k &= k - 1u)
         if (__shfl_sync(0xffffffffu, page, __ffs(k) - 1) == mine) free = false;
     const unsigned offers = __ballot_sync(0xffffffffu, free), needs = __ballot_sync(0xffffffffu, in && !keeps);

@@ -84,7 +84,7 @@ def select(logits: torch.Tensor, scores: torch.Tensor, beams: int, stop_ids: Opt
     room = torch.empty(at + R * (-(-V // TILE)) * PART, dtype=torch.int32, device=logits.device)
     base = room.data_ptr()
     _call(_fn("ti_beam_select", [P, L, I, I, I, P, I, P, I, I, P, P, P, P]),
-          logits.data_ptr(), logits.stride(0), G, held, V, scores.data_ptr(), beams, _ptr(stop_ids), n_stops, 1 if ending else 0,
+          logits.data_ptr(), logits.stride(0) if R > 1 else V, G, held, V, scores.data_ptr(), beams, _ptr(stop_ids), n_stops, 1 if ending else 0,
           base, base + 8 * n, base + 4 * at, _stream(), launches=2)
     scores, ended_scores, parents, tokens, ended_parents, ended_tokens = room[:6 * n].view(6, G, beams).unbind(0)
     return Choice(scores.view(torch.float32), parents, tokens, ended_scores.view(torch.float32), ended_parents, ended_tokens)
