@@ -420,88 +420,9 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
             n = n_found;
         }
     }
-    if (n <= ROOM) {
-#pragma unroll 1
-        for (int i = tid; i < n; i += MT) {
-            const int b = (int)(found_at[i] >> 32);
-            double total;
-            // (one that is no candidate, a NaN's neighbour at -infinity: behind all others, and told apart below)
-            if (candidate(b, __uint_as_float((unsigned)found_key[i]), total)) put(i, total, b, (int)found_at[i]);
-            else found_key[i] = 0ull;
-        }
-        __syncthreads();
-    }
-    // ranks of entry i among all that were found, and among those that are no stop tokens
-    auto rank_of = [&](int i, int& rank, int& open) {
-        const unsigned long long key = found_key[i], at = found_at[i] & ~STOP;
-        rank = open = 0;
-#pragma unroll 2
-        for (int j = 0; j < n; ++j) {
-            const unsigned long long k2 = found_key[j], w2 = found_at[j];
-            const bool before = (k2 > key) | ((k2 == key) & ((w2 & ~STOP) < at));
-            rank += before;
-            open += before & (w2 < STOP);
-        }
-    };
-    if (n > ROOM) {
-        // Equal totals without end: tile by tile in the order of places, keeping what can still be chosen.
-        __syncthreads();
-        if (tid == 0) {
-            n_found = 0;
-            s_last = 0ull;               // the key of the beams-th best so far that is no stop token's; 0: fewer than that
-        }
-        for (int base = 0; base < all; base += MT) {
-            const int i = base + tid;
-            unsigned long long top_key = 0ull;
-            if (i < all && row_add[i / a.tiles] > -INFINITY && part[i].top > -INFINITY)
-                top_key = order_key(row_add[i / a.tiles] + ((double)part[i].top - row_ref[i / a.tiles]));
-            int from = 0;
-            while (true) {
-                __syncthreads();
-                if (tid == 0) s_first = MT;
-                __syncthreads();
-                // (totals equal to the last one kept come later than it: they lose)
-                if (tid >= from && top_key > s_last) atomicMin(&s_first, tid);
-                __syncthreads();
-                const int first = s_first;
-                if (first == MT) break;
-                from = first + 1;
-                const int b = (base + first) / a.tiles, at = (base + first) % a.tiles * TILE;
-                const unsigned long long last = s_last;
-                for (int c = at + tid; c < min(at + TILE, a.V); c += MT) {
-                    double total;
-                    if (candidate(b, logits[(size_t)b * a.ld + c], total) && order_key(total) > last) put(atomicAdd(&n_found, 1), total, b, c);
-                }
-                __syncthreads();
-                n = n_found;             // at most a tile and two times BEAMS_MAX
-                unsigned long long key[(ROOM + MT - 1) / MT], whose[(ROOM + MT - 1) / MT];
-                int keep = 0;
-                for (int j = 0; j * MT + tid < n; ++j) {
-                    int rank, open;
-                    rank_of(j * MT + tid, rank, open);
-                    if (found_at[j * MT + tid] < STOP ? open < a.beams : rank < a.beams) {
-                        key[keep] = found_key[j * MT + tid];
-                        whose[keep++] = found_at[j * MT + tid];
-                        if (whose[keep - 1] < STOP && open == a.beams - 1) s_last = key[keep - 1];
-                    }
-                }
-                __syncthreads();
-                if (tid == 0) n_found = 0;
-                __syncthreads();
-                for (int j = 0; j < keep; ++j) {
-                    const int to = atomicAdd(&n_found, 1);
-                    found_key[to] = key[j];
-                    found_at[to] = whose[j];
-                }
-            }
-        }
-        __syncthreads();
-        n = n_found;
-    }
-    auto place_of_rank = [&](int i, int rank, int open) {
-        const unsigned long long whose = found_at[i];
-        if (found_key[i] == 0ull) return;        // none
-        const float total = (float)total_of(found_key[i]);
+    // what has rank ``rank`` among all and ``open`` among those that are no stop tokens (whose: beam, token and the stop bit)
+    auto settle = [&](unsigned long long key, unsigned long long whose, int rank, int open) {
+        const float total = (float)total_of(key);
         if (whose < STOP) {
             if (open < a.beams) {
                 next_score[open] = total;
@@ -514,54 +435,155 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
             a.end_token[o + rank] = (int)whose;
         }
     };
-    if (n <= 256) {
-        // a warp to an entry, a lane to one it is compared with
-#pragma unroll 1
-        for (int i = warp; i < n; i += MW) {
-            const unsigned long long key = found_key[i], at = found_at[i] & ~STOP;
-            int rank = 0, open = 0;
-#pragma unroll 1
-            for (int j = lane; j - lane < n; j += 32) {
-                const unsigned long long k2 = j < n ? found_key[j] : 0ull, w2 = j < n ? found_at[j] : ~0ull;
-                const bool before = (k2 > key) | ((k2 == key) & ((w2 & ~STOP) < at));
-                rank += __popc(__ballot_sync(0xffffffffu, before));
-                open += __popc(__ballot_sync(0xffffffffu, before & (w2 < STOP)));
+    if (n <= 32) {
+        // nearly always: an entry to a lane of one warp, which has all of the rest to itself
+        if (warp != 0) return;
+        unsigned long long key = 0ull, whose = ~0ull;            // (the key of a number is never 0)
+        if (lane < n) {
+            const int b = (int)(found_at[lane] >> 32), token = (int)found_at[lane];
+            double total;
+            if (candidate(b, __uint_as_float((unsigned)found_key[lane]), total)) {
+                key = order_key(total);
+                whose = found_at[lane] | (is_stop(token) ? STOP : 0ull);
             }
-            if (lane == 0) place_of_rank(i, rank, open);
         }
-    } else {
+        int rank = 0, open = 0;
 #pragma unroll 1
-        for (int i = tid; i < n; i += MT) {
-            int rank, open;
-            rank_of(i, rank, open);
-            place_of_rank(i, rank, open);
+        for (int j = 0; j < n; ++j) {
+            const unsigned long long k2 = __shfl_sync(0xffffffffu, key, j), w2 = __shfl_sync(0xffffffffu, whose, j);
+            const bool before = (k2 > key) | ((k2 == key) & ((w2 & ~STOP) < (whose & ~STOP)));
+            rank += before;
+            open += before & (w2 < STOP);
         }
+        if (key) settle(key, whose, rank, open);
+        __syncwarp();
+    } else {
+        if (n <= ROOM) {
+#pragma unroll 1
+            for (int i = tid; i < n; i += MT) {
+                const int b = (int)(found_at[i] >> 32);
+                double total;
+                // (one that is no candidate, a NaN's neighbour at -infinity: behind all others, and told apart below)
+                if (candidate(b, __uint_as_float((unsigned)found_key[i]), total)) put(i, total, b, (int)found_at[i]);
+                else found_key[i] = 0ull;
+            }
+            __syncthreads();
+        }
+        // ranks of entry i among all that were found, and among those that are no stop tokens
+        auto rank_of = [&](int i, int& rank, int& open) {
+            const unsigned long long key = found_key[i], at = found_at[i] & ~STOP;
+            rank = open = 0;
+#pragma unroll 2
+            for (int j = 0; j < n; ++j) {
+                const unsigned long long k2 = found_key[j], w2 = found_at[j];
+                const bool before = (k2 > key) | ((k2 == key) & ((w2 & ~STOP) < at));
+                rank += before;
+                open += before & (w2 < STOP);
+            }
+        };
+        if (n > ROOM) {
+            // Equal totals without end: tile by tile in the order of places, keeping what can still be chosen.
+            __syncthreads();
+            if (tid == 0) {
+                n_found = 0;
+                s_last = 0ull;               // the key of the beams-th best so far that is no stop token's; 0: fewer than that
+            }
+            for (int base = 0; base < all; base += MT) {
+                const int i = base + tid;
+                unsigned long long top_key = 0ull;
+                if (i < all && row_add[i / a.tiles] > -INFINITY && part[i].top > -INFINITY)
+                    top_key = order_key(row_add[i / a.tiles] + ((double)part[i].top - row_ref[i / a.tiles]));
+                int from = 0;
+                while (true) {
+                    __syncthreads();
+                    if (tid == 0) s_first = MT;
+                    __syncthreads();
+                    // (totals equal to the last one kept come later than it: they lose)
+                    if (tid >= from && top_key > s_last) atomicMin(&s_first, tid);
+                    __syncthreads();
+                    const int first = s_first;
+                    if (first == MT) break;
+                    from = first + 1;
+                    const int b = (base + first) / a.tiles, at = (base + first) % a.tiles * TILE;
+                    const unsigned long long last = s_last;
+                    for (int c = at + tid; c < min(at + TILE, a.V); c += MT) {
+                        double total;
+                        if (candidate(b, logits[(size_t)b * a.ld + c], total) && order_key(total) > last) put(atomicAdd(&n_found, 1), total, b, c);
+                    }
+                    __syncthreads();
+                    n = n_found;             // at most a tile and two times BEAMS_MAX
+                    unsigned long long key[(ROOM + MT - 1) / MT], whose[(ROOM + MT - 1) / MT];
+                    int keep = 0;
+                    for (int j = 0; j * MT + tid < n; ++j) {
+                        int rank, open;
+                        rank_of(j * MT + tid, rank, open);
+                        if (found_at[j * MT + tid] < STOP ? open < a.beams : rank < a.beams) {
+                            key[keep] = found_key[j * MT + tid];
+                            whose[keep++] = found_at[j * MT + tid];
+                            if (whose[keep - 1] < STOP && open == a.beams - 1) s_last = key[keep - 1];
+                        }
+                    }
+                    __syncthreads();
+                    if (tid == 0) n_found = 0;
+                    __syncthreads();
+                    for (int j = 0; j < keep; ++j) {
+                        const int to = atomicAdd(&n_found, 1);
+                        found_key[to] = key[j];
+                        found_at[to] = whose[j];
+                    }
+                }
+            }
+            __syncthreads();
+            n = n_found;
+        }
+        if (n <= 256) {
+            // a warp to an entry, a lane to one it is compared with
+#pragma unroll 1
+            for (int i = warp; i < n; i += MW) {
+                const unsigned long long key = found_key[i], at = found_at[i] & ~STOP;
+                int rank = 0, open = 0;
+#pragma unroll 1
+                for (int j = lane; j - lane < n; j += 32) {
+                    const unsigned long long k2 = j < n ? found_key[j] : 0ull, w2 = j < n ? found_at[j] : ~0ull;
+                    const bool before = (k2 > key) | ((k2 == key) & ((w2 & ~STOP) < at));
+                    rank += __popc(__ballot_sync(0xffffffffu, before));
+                    open += __popc(__ballot_sync(0xffffffffu, before & (w2 < STOP)));
+                }
+                if (lane == 0 && key) settle(key, found_at[i], rank, open);
+            }
+        } else {
+#pragma unroll 1
+            for (int i = tid; i < n; i += MT) {
+                int rank, open;
+                rank_of(i, rank, open);
+                if (found_key[i]) settle(found_key[i], found_at[i], rank, open);
+            }
+        }
+        __syncthreads();
+        if (warp != 0) return;
     }
-    __syncthreads();
     // Placement by one warp, a lane per rank: the first child of a beam stays at its parent's place, the others take the places of
     // the beams without a child, in order.  What is copied is then never what another copy overwrites.
-    if (warp == 0) {
-        const int p = next_parent[lane];
-        const bool there = p >= 0;
-        const unsigned below = (1u << lane) - 1u;
-        const unsigned same = __match_any_sync(0xffffffffu, p);
-        const bool stays = there && (same & below) == 0u;
-        const unsigned kept = __reduce_or_sync(0xffffffffu, stays ? 1u << p : 0u);
-        const unsigned goes = __ballot_sync(0xffffffffu, there && !stays);
-        if (!((kept >> lane) & 1u)) free_place[__popc(~kept & below)] = lane;
-        __syncwarp();
-        const int place = stays ? p : there ? free_place[__popc(goes & below)] : -1;
-        const unsigned taken = __reduce_or_sync(0xffffffffu, place >= 0 ? 1u << place : 0u);
-        if (place >= 0) {
-            a.out_score[o + place] = next_score[lane];
-            a.out_parent[o + place] = p;
-            a.out_token[o + place] = next_token[lane];
-        }
-        if (lane < a.beams && !((taken >> lane) & 1u)) {
-            a.out_score[o + lane] = -INFINITY;
-            a.out_parent[o + lane] = lane;
-            a.out_token[o + lane] = 0;
-        }
+    const int p = next_parent[lane];
+    const bool there = p >= 0;
+    const unsigned below = (1u << lane) - 1u;
+    const unsigned same = __match_any_sync(0xffffffffu, p);
+    const bool stays = there && (same & below) == 0u;
+    const unsigned kept = __reduce_or_sync(0xffffffffu, stays ? 1u << p : 0u);
+    const unsigned goes = __ballot_sync(0xffffffffu, there && !stays);
+    if (!((kept >> lane) & 1u)) free_place[__popc(~kept & below)] = lane;
+    __syncwarp();
+    const int place = stays ? p : there ? free_place[__popc(goes & below)] : -1;
+    const unsigned taken = __reduce_or_sync(0xffffffffu, place >= 0 ? 1u << place : 0u);
+    if (place >= 0) {
+        a.out_score[o + place] = next_score[lane];
+        a.out_parent[o + place] = p;
+        a.out_token[o + place] = next_token[lane];
+    }
+    if (lane < a.beams && !((taken >> lane) & 1u)) {
+        a.out_score[o + lane] = -INFINITY;
+        a.out_parent[o + lane] = lane;
+        a.out_token[o + lane] = 0;
     }
 }
 }  // namespace
