@@ -96,6 +96,23 @@ def test_select_values(kind, V):
     check_select(x, s, B, [1, 7])
 
 
+@pytest.mark.parametrize("V", [700, 40000, 151936])
+@pytest.mark.parametrize("width,shift", [(0.3, 0.0), (2.5, 0.0), (8.0, 30.0), (2.5, -60.0), (3.0, 150.0), (30.0, -20.0)])
+def test_select_near_ties_between_rows(V, width, shift):
+    """Beams whose rows hold the same logits in another order, and whose scores differ by one step of 32 bits: each token's totals in
+    the two rows are 6e-8 apart, sixty times what the rows' sums may be off by (1e-9 of a term, csrc/beam_select.cu)."""
+    G, B = 3, 6
+    g = torch.Generator(device=DEV).manual_seed(V)
+    base = torch.randn(V, generator=g, device=DEV) * width + shift
+    x = torch.stack([base[torch.randperm(V, generator=g, device=DEV)] for _ in range(G * B)])
+    one = torch.tensor(-0.75)
+    steps = [one]
+    for _ in range(B - 1):
+        steps.append(torch.nextafter(steps[-1], torch.tensor(0.0)))
+    s = torch.stack([torch.stack(steps)[torch.randperm(B)] for _ in range(G)]).to(DEV)
+    check_select(x, s, B, [3])
+
+
 def test_select_masks_and_missing_beams():
     inf, nan = float("inf"), float("nan")
     x, s = inputs(4, 4, 700, seed=9)
