@@ -21,6 +21,9 @@ from .wide import _fn
 from ..cache.allocators import PAGE
 
 P, I, L = c_void_p, c_int, c_longlong
+_SELECT = [P, L, I, I, I, P, I, P, I, I, P, P, P, P]
+_TABLES = [P, I, P, P, P, I, I, I, I, I, P, P]
+_REORDER = [P, I, I, P, P, P, I, P]
 BEAMS_MAX = 32          # beams of one group
 STOPS_MAX = 16          # stop tokens
 TABLES_MAX = 8          # page tables of one cache
@@ -83,10 +86,10 @@ def select(logits: torch.Tensor, scores: torch.Tensor, beams: int, stop_ids: Opt
     at = (6 * n + 3) & ~3
     room = torch.empty(at + R * (-(-V // TILE)) * PART, dtype=torch.int32, device=logits.device)
     base = room.data_ptr()
-    _call(_fn("ti_beam_select", [P, L, I, I, I, P, I, P, I, I, P, P, P, P]),
+    _call(_fn("ti_beam_select", _SELECT),
           logits.data_ptr(), logits.stride(0) if R > 1 else V, G, held, V, scores.data_ptr(), beams, _ptr(stop_ids), n_stops, 1 if ending else 0,
           base, base + 8 * n, base + 4 * at, _stream(), launches=2)
-    scores, ended_scores, parents, tokens, ended_parents, ended_tokens = room[:6 * n].view(6, G, beams).unbind(0)
+    scores, ended_scores, parents, tokens, ended_parents, ended_tokens = room.as_strided((6, G, beams), (n, beams, 1)).unbind(0)
     return Choice(scores.view(torch.float32), parents, tokens, ended_scores.view(torch.float32), ended_parents, ended_tokens)
 
 
@@ -131,7 +134,7 @@ def tables(slots: torch.Tensor, parents: torch.Tensor, lengths: torch.Tensor, ex
         n_slots = shape[0]
         words += (table.data_ptr(), home.data_ptr(), shape[1], ring_rows // PAGE)
     moves = torch.empty((1 + n_tables, G * B, 3), dtype=torch.int32, device=slots.device)
-    _call(_fn("ti_beam_tables", [P, I, P, P, P, I, I, I, I, I, P, P]), (c_longlong * len(words))(*words), n_tables, slots.data_ptr(),
+    _call(_fn("ti_beam_tables", _TABLES), (c_longlong * len(words))(*words), n_tables, slots.data_ptr(),
           parents.data_ptr(), lengths.data_ptr(), int(extra), G, B, PAGE, n_slots if n_slots is not None else 1 << 30, moves.data_ptr(),
           _stream(), launches=max(1, -(-n_tables // 4)))
     return moves
@@ -191,5 +194,5 @@ def reorder(areas: Areas, moves: torch.Tensor) -> None:
     if areas.n_areas == 0:
         return
     _here(moves, areas.records, what="beam reorder")
-    _call(_fn("ti_beam_reorder", [P, I, I, P, P, P, I, P]), _ptr(areas.records), areas.n_areas, lists, areas._first, areas._pieces,
+    _call(_fn("ti_beam_reorder", _REORDER), _ptr(areas.records), areas.n_areas, lists, areas._first, areas._pieces,
           moves.data_ptr(), shape[1], _stream())
