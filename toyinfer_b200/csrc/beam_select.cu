@@ -16,8 +16,8 @@
 // are taken one by one in the order of (b, v), each cut down to the best so far: an equal total that comes later loses, so that
 // tiles which only reach the bound are passed over from then on.
 //
-// Totals and the order are in 64 bits, and a row's sum is good to 1e-9: beams compete by sums over a whole vocabulary, and at 32 bits
-// the order of two candidates of different rows would depend on how the sums were split.
+// Totals, sums and the order are in 64 bits, a sum good to 5e-11: beams compete by sums over a whole vocabulary, and at 32 bits the
+// order of two candidates of different rows would depend on how the sums were split.
 #include "common.cuh"
 
 namespace {
@@ -34,7 +34,8 @@ constexpr int KEYS = 3840;           // tiles of a group whose totals are kept i
 constexpr int AHEAD = 4;             // pairs of tiles on the way at a time, when they are read again
 constexpr int HELD = 5;              // tiles of a row, of 32 each, whose parts a warp has on the way at a time
 constexpr float BIG = 3.402823466e38f;
-constexpr float LOW = -40.f, HIGH = 80.f;       // a tile's exponentials are summed as they are while its largest logit lies here
+constexpr float PLAIN = 600.f;       // |largest logit| of a tile up to which its exponentials are summed as they are
+constexpr float LEAST = -690.f;      // what lies below counts as this: e^-690, next to nothing beside e^-600
 constexpr unsigned KEY_NONE = 0x007FFFFFu;      // the key of -infinity: the least key of all
 
 __device__ __forceinline__ unsigned order_key(float x) {
@@ -58,60 +59,25 @@ __constant__ double pow16[16] = {1.0, 1.0442737824274138, 1.0905077326652577, 1.
                                  1.2968395546510096, 1.3542555469368927, 1.4142135623730951, 1.4768261459394993, 1.5422108254079407,
                                  1.6104903319492543, 1.681792830507429, 1.7562521603732995, 1.8340080864093424, 1.9152065613971474};
 
-// exp after Tang, "Table-driven implementation of the exponential function in IEEE floating-point arithmetic", 1989: x =
-// (16 n + j) ln 2 / 16 + r with |r| <= ln 2 / 32, exp(x) = 2^n 2^(j/16) (1 + q), q = r + r^2/2 + r^3/6 + r^4/24 (the rest is at most
-// 4e-11).  k = 16 n + j is rounded by adding a number whose last bits are then k; ``table`` holds 2^(j/16) with j taken off bit 16 on
-// of its high word, so that adding k << 16 there multiplies by 2^n.
-//
-// Two values at a time, -80 <= x <= 80 (smaller ones count as -80; larger ones give anything).  q is formed in 32 bits, of an r that is
-// exact but for its last rounding (the high part of ln 2 / 16 has 21 bits, and the first step cancels to an exact number); what enters
-// the sum in 32 bits is the share q <= 0.022 of each term, the 2^(j/16) 2^n enter in 64: an error of 1e-9 of a term at most.  Fewer
-// instructions than the form in 64 bits below it: 64 rows of 151,936 logits take 9.5 us instead of 10.9; 7.2 with no exponential.
-typedef unsigned long long f32x2;
-__device__ __forceinline__ f32x2 pack(float a, float b) { f32x2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
-__device__ __forceinline__ void unpack(f32x2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ f32x2 both(float a) { return pack(a, a); }
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) { f32x2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
-__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) { f32x2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) { f32x2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
-
-__device__ __forceinline__ double scaled(const double* __restrict__ table, int k) {
-    const double f = table[k & 15];
-    return __hiloint2double(__double2hiint(f) + (int)((unsigned)k << 16), __double2loint(f));
-}
-// its leading 24 bits as a float (within the range of one)
-__device__ __forceinline__ float leading(double f) {
-    return __uint_as_float(__funnelshift_l((unsigned)__double2loint(f), (unsigned)__double2hiint(f), 3) + 0x40000000u);
-}
-
-// s0 + s1 + rest grow by exp(x0) + exp(x1)
-__device__ __forceinline__ void add_exps(double& s0, double& s1, f32x2& rest, float x0, float x1, const double* __restrict__ table) {
-    const f32x2 x = pack(fmaxf(x0, -80.f), fmaxf(x1, -80.f));          // (a NaN counts as -80 too)
-    const f32x2 t = fma2(x, both(23.0831206542f), both(12582912.f));   // 16 / ln 2, and 1.5 * 2^23
-    const f32x2 kr = add2(t, both(-12582912.f));
-    const f32x2 r = fma2(kr, both(0x1.05c61p-33f), fma2(kr, both(-0x1.62e43p-5f), x));       // - ln 2 / 16 in two parts
-    const f32x2 q = fma2(mul2(r, r), fma2(r, fma2(r, both(1.f / 24.f), both(1.f / 6.f)), both(0.5f)), r);
-    float t0, t1;
-    unpack(t, t0, t1);
-    const double f0 = scaled(table, __float_as_int(t0)), f1 = scaled(table, __float_as_int(t1));
-    s0 += f0;
-    s1 += f1;
-    rest = fma2(pack(leading(f0), leading(f1)), q, rest);
-}
-
-// sum + exp(x), x <= 690, all in 64 bits
+// sum + exp(x), -690 <= x <= 690 (a larger one gives anything), relative error below 5e-11; after Tang, "Table-driven implementation of
+// the exponential function in IEEE floating-point arithmetic", 1989: x = (16 n + j) ln 2 / 16 + r with |r| <= ln 2 / 32, exp(x) =
+// 2^n 2^(j/16) exp(r), and exp(r) - 1 - r - ... - r^4/24 is at most r^5 / 120 = 4e-11.  k = 16 n + j is rounded by adding 1.5 * 2^52, whose
+// last bits are then k; ``table`` holds 2^(j/16) with j taken off bit 16 on of its high word, so that adding k << 16 there multiplies by
+// 2^n.  Eight operations of 64 bits: 64 rows of 151,936 logits take 11.0 us, 15.8 with exp(), 7.2 with no exponential.  (With r and the
+// polynomial in 32 bits, two values at a time, 9.5, but a sum in which one term prevails is then good to 1e-8 only.)
 __device__ __forceinline__ double add_exp(double sum, double x, const double* __restrict__ table) {
-    x = fmax(x, -690.0);                                                // (a NaN counts as -690 too)
-    const double t = fma(x, 23.083120654223414, 6755399441055744.0);   // 1.5 * 2^52
+    const double t = fma(x, 23.083120654223414, 6755399441055744.0);
+    const int k = __double2loint(t);
     const double r = fma(t - 6755399441055744.0, -0.04332169878499658, x);
     const double p = fma(r, fma(r, fma(r, fma(r, 1.0 / 24.0, 1.0 / 6.0), 0.5), 1.0), 1.0);
-    return fma(scaled(table, __double2loint(t)), p, sum);
+    const double f = table[k & 15];
+    return fma(__hiloint2double(__double2hiint(f) + (int)((unsigned)k << 16), __double2loint(f)), p, sum);
 }
 
 struct __align__(16) Part {              // of a tile
     double sum;          // of exp(x - ref)
     float top;           // the largest logit; -infinity: none, and the rest is not written
-    float ref;           // 0, or ``top`` where that is below LOW or above HIGH
+    float ref;           // 0, or ``top`` where the exponentials would leave the range of 64 bits
 };
 
 struct ScanArgs {
@@ -162,24 +128,20 @@ __global__ void __launch_bounds__(SCAN_WARPS * 32, 16) beam_scan_kernel(ScanArgs
     load_tile<VEC>(v, x, tile * TILE, a.V, lane);
     float top = -INFINITY;
     double s[4] = {0.0, 0.0, 0.0, 0.0};
-    f32x2 rest[2] = {both(0.f), both(0.f)};
 #pragma unroll
-    for (int e = 0; e < LANE; e += 2) {
-        top = fmaxf(top, fmaxf(v[e], v[e + 1]));              // (a NaN is passed over)
-        add_exps(s[e & 2], s[(e & 2) + 1], rest[(e >> 1) & 1], v[e], v[e + 1], table);
+    for (int e = 0; e < LANE; ++e) {
+        top = fmaxf(top, v[e]);              // (a NaN is passed over, and counts as LEAST below)
+        s[e & 3] = add_exp(s[e & 3], (double)fmaxf(v[e], LEAST), table);
     }
     top = warp_max(fminf(top, BIG));
-    const bool plain = top >= LOW && top <= HIGH;
+    const bool plain = fabsf(top) <= PLAIN;
     if (!plain && top > -INFINITY) {
         s[0] = s[1] = s[2] = s[3] = 0.0;
-        rest[0] = rest[1] = both(0.f);
 #pragma unroll
-        for (int e = 0; e < LANE; ++e) s[e & 3] = add_exp(s[e & 3], (double)fminf(v[e], v[e] == v[e] ? BIG : -BIG) - (double)top, table);
+        for (int e = 0; e < LANE; ++e)
+            if (v[e] > -INFINITY) s[e & 3] = add_exp(s[e & 3], fmax((double)fminf(v[e], BIG) - (double)top, (double)LEAST), table);
     }
-    float r[4];
-    unpack(rest[0], r[0], r[1]);
-    unpack(rest[1], r[2], r[3]);
-    double sum = ((s[0] + s[1]) + (s[2] + s[3])) + ((double)(r[0] + r[1]) + (double)(r[2] + r[3]));
+    double sum = (s[0] + s[1]) + (s[2] + s[3]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) a.part[(size_t)row * a.tiles + tile] = Part{sum, top, plain ? 0.f : top};
