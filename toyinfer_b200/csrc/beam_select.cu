@@ -26,12 +26,13 @@ constexpr int STOPS_MAX = 16;
 constexpr int TILE = 1024;           // logits that a warp takes
 constexpr int LANE = TILE / 32;
 constexpr int SCAN_WARPS = 2;        // a scan block's; warps that share nothing but the table, so small blocks leave no SM waiting
-constexpr int MT = 512;              // threads of a merge block
+constexpr int MT = 1024;             // threads of a merge block
 constexpr int MW = MT / 32;
+constexpr int SIDES = MT / 256;      // tiles that are read again side by side
 constexpr int TILES = 512;           // tiles of a group that may reach the bound
 constexpr int ROOM = 1536;           // candidates above it; more than a tile and all that is kept of the ones before
 constexpr int KEYS = 3840;           // tiles of a group whose totals are kept in shared memory
-constexpr int AHEAD = 4;             // pairs of tiles on the way at a time, when they are read again
+constexpr int AHEAD = 2;             // tiles that each side has on the way at a time
 constexpr int HELD = 5;              // tiles of a row, of 32 each, whose parts a warp has on the way at a time
 constexpr float BIG = 3.402823466e38f;
 constexpr float PLAIN = 600.f;       // |largest logit| of a tile up to which its exponentials are summed as they are
@@ -197,7 +198,8 @@ struct MergeArgs {
 };
 
 // What a block of the merge spends is latency: instructions that a block runs once come from L2 as its data do, so the code is kept
-// in loops, and what is rare is out of the way.
+// in loops, and what is rare is out of the way.  Behind the scan it takes 4.8 us for one row of 151,936, 5 for a group of four, 10 for
+// 24 rows of 123,373 at odd addresses (12 with 512 threads, 17 with 256; one row then 0.5 us less).
 template <bool VEC>
 __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
     ti_pdl_trigger();
@@ -357,12 +359,12 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
     const int listed = n_tiles;
     auto each = [&](auto&& f) {
 #pragma unroll 1
-        for (int i0 = tid >> 8; i0 < listed; i0 += 2 * AHEAD) {          // half of the block to a tile, four logits a thread
+        for (int i0 = tid >> 8; i0 < listed; i0 += SIDES * AHEAD) {      // 256 threads to a tile, four logits each
             const int part_of = tid & 255;
             float v[AHEAD][4];
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
-                const int what = tile_list[min(i0 + 2 * u, listed - 1)];
+                const int what = tile_list[min(i0 + SIDES * u, listed - 1)];
                 const float* x = logits + (size_t)(what >> 24) * a.ld;
                 const int at = (what & 0xFFFFFF) * TILE;
                 if (VEC && at + TILE <= a.V) {
@@ -378,8 +380,8 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
             }
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
-                if (i0 + 2 * u >= listed) continue;
-                const int what = tile_list[i0 + 2 * u], b = what >> 24, at = (what & 0xFFFFFF) * TILE;
+                if (i0 + SIDES * u >= listed) continue;
+                const int what = tile_list[i0 + SIDES * u], b = what >> 24, at = (what & 0xFFFFFF) * TILE;
                 const float cut = row_cut[b];
                 unsigned hits = 0u;
 #pragma unroll
