@@ -11,9 +11,9 @@ its tokens, but of its score and of the count that its value divides by), after 
 ``max_seq_len`` positions.
 
 The loop only decides.  It runs steps through a ``stepper`` with ``open(prompt, length) -> slots``, ``close(slots)``,
-``prompt(entries, want) -> rows``, ``stack(rows) -> logits``, ``begin(groups)``, ``select(logits, scores, drawn) -> choice``,
-``step(slots, choice, groups) -> logits``, ``read(choice)``, ``tokens_needed(prompt, length)`` and ``keep(choice or logits,
-groups)``, so that its decisions can be tested without a device.
+``tokens_needed(prompt, length)``, ``prompt(entries, want) -> logits``, ``stack(rows) -> logits``, ``begin(groups)``,
+``select(logits, scores, drawn) -> choice``, ``step(slots, choice, groups) -> logits``, ``read(choice)``, ``keep(logits,
+groups)`` and ``carry(choice, groups) -> scores``, so that its decisions can be tested without a device.
 
 The reference runs the whole prefix again for every beam and step (src/engine_runtime.cpp:472-569).
 """

@@ -34,11 +34,12 @@ PIECE = 16384           # bytes that a warp moves at a time (csrc/beam_reorder.c
 
 def _here(*tensors, what: str) -> None:
     """All on the current device: the launch goes to its stream."""
+    devices = {t.get_device() for t in tensors if t is not None}
+    if -1 in devices:                    # not a CUDA device
+        _need_cuda(*tensors, what=what)
     now = _raw_device() if _raw_device is not None else torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and t.get_device() != now:          # (-1: not a CUDA device)
-            _need_cuda(t, what=what)
-            raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{now}")
+    if devices - {now}:
+        raise KernelError(f"{what}: tensors on cuda {sorted(devices)}, the current device is cuda:{now}")
 
 
 class Choice(NamedTuple):
