@@ -198,8 +198,8 @@ struct MergeArgs {
 };
 
 // What a block of the merge spends is latency: instructions that a block runs once come from L2 as its data do, so the code is kept
-// in loops, and what is rare is out of the way.  Behind the scan it takes 4.8 us for one row of 151,936, 5 for a group of four, 10 for
-// 24 rows of 123,373 at odd addresses (12 with 512 threads, 17 with 256; one row then 0.5 us less).
+// in loops, and what is rare is out of the way.  Behind the scan it takes 5 us for one row of 151,936 as for a group of four, 10
+// for 24 rows of 123,373 at odd addresses (12 with 512 threads, 19 with 256; one row 0.5 us less with 512).
 template <bool VEC>
 __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
     ti_pdl_trigger();

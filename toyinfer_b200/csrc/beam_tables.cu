@@ -15,7 +15,8 @@
 // tables or twice in a group, and homes without a page per beam are reported in the status word and left out.
 //
 // A block per group and table.  Everything here is a few KB: what counts is the launch and the chain of loads behind it (parents,
-// then rows, then the pages of column w), so all tables of a cache take one launch and a row is copied by a warp.
+// then rows, then the pages of column w), so all tables of a cache take one launch and a row is copied by a warp: 2.4 us for one request
+// of four beams, 4.0 for 64 of eight over two tables of 128 and 16 columns (4.2 and 7.4 with a block per group for all its tables).
 #include "tma.cuh"
 
 namespace {

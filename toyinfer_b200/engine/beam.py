@@ -78,7 +78,7 @@ class _Search:
         """Takes in one selection; True while the search goes on."""
         drawn = len(self.tokens)
         for score, parent in zip(ended_scores, ended_parents):
-            if parent >= 0:
+            if parent >= 0 and score > float("-inf"):
                 h = Hypothesis([], score, self._value(score, drawn + 1), "stop")
                 # worse than everything in a full list: its tokens need not be read back
                 if len(self.ended) < self.params.beams or h.value > self.ended[-1].value:
