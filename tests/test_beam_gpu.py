@@ -44,7 +44,8 @@ def inputs(G, held, V, seed=0, pad=0, width=2.5):
 @pytest.mark.parametrize("G,held,B,V,n_stops,pad", [
     (1, 1, 1, 1, 0, 0), (1, 1, 4, 2, 0, 0), (1, 1, 8, 5, 2, 0), (2, 3, 3, 7, 1, 3), (3, 4, 4, 520, 1, 0), (5, 2, 7, 1023, 3, 1),
     (1, 4, 4, 8192, 1, 0), (1, 4, 4, 8193, 1, 0), (2, 5, 5, 8191, 0, 1), (4, 4, 4, 32000, 2, 0), (2, 8, 8, 16384, 2, 4),
-    (1, 1, 32, 20001, 16, 0), (2, 32, 32, 9001, 16, 2), (3, 24, 24, 4099, 5, 0), (1, 4, 4, 151936, 1, 0), (70, 3, 3, 300, 1, 0)])
+    (1, 1, 32, 20001, 16, 0), (2, 32, 32, 9001, 16, 2), (3, 24, 24, 4099, 5, 0), (1, 4, 4, 151936, 1, 0), (70, 3, 3, 300, 1, 0),
+    (3000, 4, 4, 130, 1, 1)])
 def test_select_sizes(G, held, B, V, n_stops, pad):
     x, s = inputs(G, held, V, seed=V + G, pad=pad)
     rng = np.random.RandomState(V)
@@ -482,7 +483,8 @@ def test_refusals():
     from toyinfer_b200.kernels import beam as KB
     x, s = inputs(2, 3, 40)
     ids = torch.zeros(17, dtype=torch.int32, device=DEV)
-    for args in ((x.double(), s, 3), (x.t(), s, 3), (x, s.double(), 3), (x[:5], s, 3), (x, s, 2), (x, s, 33), (x, s.t(), 3), (x, s, 3, ids),
+    many = torch.zeros(70000, 2, device=DEV)
+    for args in ((many, torch.zeros(17500, 4, device=DEV), 4), (x.double(), s, 3), (x.t(), s, 3), (x, s.double(), 3), (x[:5], s, 3), (x, s, 2), (x, s, 33), (x, s.t(), 3), (x, s, 3, ids),
                  (x, s, 3, ids[:2].long()), (x.cpu(), s, 3), (x[:, :0], s, 3), (x, s[:0], 3)):
         with pytest.raises(K.KernelError):
             KB.select(*args)

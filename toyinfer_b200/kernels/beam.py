@@ -110,7 +110,8 @@ def tables(slots: torch.Tensor, parents: torch.Tensor, lengths: torch.Tensor, ex
     slots and parents int32 [groups, beams], parents as ``select`` gives them; lengths int32 [groups]: the positions that each
     group's sequences hold are lengths + extra.  A page that is not written any more is shared by the places that come from its
     beam; at the column that the next token goes to every place gets a page of its own, out of the group's homes there, and the
-    rows that it holds so far are among the moves.  At that column the homes of a group are pages of its own, one per place."""
+    rows that it holds so far are among the moves.  At that column the homes of a group are pages of its own, one per place.
+    ``reorder`` comes next, before anything reads the tables or writes the pages."""
     _here(slots, parents, lengths, what="beam tables")
     for t, what in ((slots, "slots"), (parents, "parents"), (lengths, "lengths")):
         if t.dtype != torch.int32 or not t.is_contiguous():
