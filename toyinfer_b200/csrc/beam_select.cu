@@ -17,7 +17,8 @@
 // tiles which only reach the bound are passed over from then on.
 //
 // Totals, sums and the order are in 64 bits, a sum good to 5e-11: beams compete by sums over a whole vocabulary, and at 32 bits the
-// order of two candidates of different rows would depend on how the sums were split.
+// order of two candidates of different rows would depend on how the sums were split.  Scores come and go in 32 or in 64 bits: a search
+// that hands them over in 32 rounds the whole sum at every step, 3e-2 after 8,000 tokens.
 #include "common.cuh"
 
 namespace {
@@ -81,11 +82,25 @@ struct __align__(16) Part {              // of a tile
     float ref;           // 0, or ``top`` where the exponentials would leave the range of 64 bits
 };
 
+// Scores are float32 or float64, as the caller has them.
+struct Scores {
+    const void* at;
+    int wide;
+};
+__device__ __forceinline__ double score_at(Scores s, size_t i) {
+    const void* p = ti_dependent(s.at);
+    return s.wide ? static_cast<const double*>(p)[i] : (double)static_cast<const float*>(p)[i];
+}
+__device__ __forceinline__ void put_score(void* out, int wide, size_t i, double score) {
+    if (wide) static_cast<double*>(out)[i] = score;
+    else static_cast<float*>(out)[i] = (float)score;
+}
+
 struct ScanArgs {
     const float* logits;
     long long ld;
     int V, tiles;
-    const float* scores;
+    Scores scores;
     Part* part;          // [rows, tiles]
 };
 
@@ -122,9 +137,8 @@ __global__ void __launch_bounds__(SCAN_WARPS * 32, 16) beam_scan_kernel(ScanArgs
         table[threadIdx.x] = __hiloint2double(__double2hiint(pow16[threadIdx.x]) - ((int)threadIdx.x << 16), __double2loint(pow16[threadIdx.x]));
     __syncthreads();
     ti_pdl_sync();
-    const float* scores = ti_dependent(a.scores);
     const float* x = ti_dependent(a.logits) + (size_t)row * a.ld;
-    if (tile >= a.tiles || !(scores[row] > -INFINITY)) return;      // (the merge leaves such a row out as well)
+    if (tile >= a.tiles || !(score_at(a.scores, row) > -INFINITY)) return;      // (the merge leaves such a row out as well)
     float v[LANE];
     load_tile<VEC>(v, x, tile * TILE, a.V, lane);
     float top = -INFINITY;
@@ -185,14 +199,14 @@ __device__ __forceinline__ unsigned bound_of(const unsigned* __restrict__ keys, 
 struct MergeArgs {
     const float* logits;
     long long ld;
-    const float* scores;     // [groups, held]
+    Scores scores;           // [groups, held]
     const Part* part;
     const int* stops;
     int held, beams, n_stops, tiles, V, ending;
-    float* out_score;        // [groups, beams], by place
+    void* out_score;         // [groups, beams], by place, of the type of ``scores`` as ``end_score`` is
     int* out_parent;
     int* out_token;
-    float* end_score;        // [groups, beams], by rank
+    void* end_score;         // [groups, beams], by rank
     int* end_parent;
     int* end_token;
 };
@@ -210,7 +224,7 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
     __shared__ int tile_list[TILES];                                 // beam << 24 | tile
     __shared__ double row_add[BEAMS_MAX], row_ref[BEAMS_MAX];        // a total is row_add + (x - row_ref); row_add -infinity: no beam
     __shared__ float row_cut[BEAMS_MAX];                             // logits below it do not reach the bound
-    __shared__ float next_score[BEAMS_MAX];
+    __shared__ double next_score[BEAMS_MAX];
     __shared__ int next_parent[BEAMS_MAX], next_token[BEAMS_MAX], free_place[BEAMS_MAX];
     __shared__ int stops[STOPS_MAX];
     __shared__ int n_tiles, n_found, s_first;
@@ -226,14 +240,13 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
     }
     if (tid == 0) n_tiles = n_found = 0;
     ti_pdl_sync();
-    const float* scores = ti_dependent(a.scores) + (size_t)g * a.held;
     const float* logits = ti_dependent(a.logits) + (size_t)g * a.held * a.ld;
     const Part* part = ti_dependent(a.part) + (size_t)g * all;
     const int* stop_ids = ti_dependent(a.stops);
     const size_t o = (size_t)g * a.beams;
     if (tid < a.n_stops) stops[tid] = stop_ids[tid];
     if (tid < a.beams) {
-        a.end_score[o + tid] = -INFINITY;
+        put_score(a.end_score, a.scores.wide, o + tid, -INFINITY);
         a.end_parent[o + tid] = -1;
         a.end_token[o + tid] = -1;
     }
@@ -256,7 +269,7 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
 #pragma unroll 1
     for (int b = warp; b < a.held; b += MW) {
         const Part* p = part + (size_t)b * a.tiles;
-        const float score = scores[b];
+        const double score = score_at(a.scores, (size_t)g * a.held + b);
         bool some = false, shifted = false;
         double sum = 0.0;
         Part q[HELD];
@@ -288,7 +301,7 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
         }
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        const double add = there ? (double)score - log(sum) : -INFINITY, ref = m;
+        const double add = there ? score - log(sum) : -INFINITY, ref = m;
         if (lane == 0) {
             row_add[b] = add;
             row_ref[b] = ref;
@@ -426,7 +439,7 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
     }
     // what has rank ``rank`` among all and ``open`` among those that are no stop tokens (whose: beam, token and the stop bit)
     auto settle = [&](unsigned long long key, unsigned long long whose, int rank, int open) {
-        const float total = (float)total_of(key);
+        const double total = total_of(key);
         if (whose < STOP) {
             if (open < a.beams) {
                 next_score[open] = total;
@@ -434,7 +447,7 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
                 next_token[open] = (int)whose;
             }
         } else if (a.ending && rank < a.beams) {
-            a.end_score[o + rank] = total;
+            put_score(a.end_score, a.scores.wide, o + rank, total);
             a.end_parent[o + rank] = (int)((whose & ~STOP) >> 32);
             a.end_token[o + rank] = (int)whose;
         }
@@ -580,22 +593,22 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
     const int place = stays ? p : there ? free_place[__popc(goes & below)] : -1;
     const unsigned taken = __reduce_or_sync(0xffffffffu, place >= 0 ? 1u << place : 0u);
     if (place >= 0) {
-        a.out_score[o + place] = next_score[lane];
+        put_score(a.out_score, a.scores.wide, o + place, next_score[lane]);
         a.out_parent[o + place] = p;
         a.out_token[o + place] = next_token[lane];
     }
     if (lane < a.beams && !((taken >> lane) & 1u)) {
-        a.out_score[o + lane] = -INFINITY;
+        put_score(a.out_score, a.scores.wide, o + lane, -INFINITY);
         a.out_parent[o + lane] = lane;
         a.out_token[o + lane] = 0;
     }
 }
 }  // namespace
 
-// out_scores [2, groups, beams]: the next beams' and the ended ones'; out_places [4, groups, beams]: parents, tokens, and of the
+// scores, and out_scores [2, groups, beams] (the next beams' and the ended ones'): float64 where wide_scores, float32 otherwise; out_places [4, groups, beams]: parents, tokens, and of the
 // ended ones parents and tokens; scratch: a Part for every tile of 1,024 logits of every row.
-extern "C" int ti_beam_select(const float* logits, long long ld, int groups, int held, int V, const float* scores, int beams,
-                              const int* stops, int n_stops, int ending, float* out_scores, int* out_places, void* scratch,
+extern "C" int ti_beam_select(const float* logits, long long ld, int groups, int held, int V, const void* scores, int wide_scores,
+                              int beams, const int* stops, int n_stops, int ending, void* out_scores, int* out_places, void* scratch,
                               cudaStream_t stream) {
     TI_REQUIRE(groups >= 1 && held >= 1 && V >= 1 && ld >= V, "beam select: %d groups of %d rows of %d logits, %lld apart", groups, held, V, ld);
     TI_REQUIRE(beams >= 1 && beams <= BEAMS_MAX && held <= beams, "beam select: %d beams from %d (at most %d, and no fewer than before)",
@@ -607,12 +620,14 @@ extern "C" int ti_beam_select(const float* logits, long long ld, int groups, int
     const int tiles = (V + TILE - 1) / TILE;
     TI_REQUIRE(tiles < 1 << 24, "beam select: %d logits a row", V);
     const bool vec = ld % 4 == 0 && (reinterpret_cast<uintptr_t>(logits) & 15) == 0;
-    ScanArgs s = {logits, ld, V, tiles, scores, static_cast<Part*>(scratch)};
+    const Scores from = {scores, wide_scores};
+    ScanArgs s = {logits, ld, V, tiles, from, static_cast<Part*>(scratch)};
     const dim3 grid((tiles + SCAN_WARPS - 1) / SCAN_WARPS, (unsigned)rows);
     TI_CUDA(ti_launch(vec ? beam_scan_kernel<true> : beam_scan_kernel<false>, grid, dim3(SCAN_WARPS * 32), 0, stream, s));
     const size_t n = (size_t)groups * beams;
-    MergeArgs m = {logits, ld, scores, s.part, stops, held, beams, n_stops, tiles, V, ending,
-                   out_scores, out_places, out_places + n, out_scores + n, out_places + 2 * n, out_places + 3 * n};
+    void* ended = static_cast<char*>(out_scores) + n * (wide_scores ? 8 : 4);
+    MergeArgs m = {logits, ld, from, s.part, stops, held, beams, n_stops, tiles, V, ending,
+                   out_scores, out_places, out_places + n, ended, out_places + 2 * n, out_places + 3 * n};
     TI_CUDA(ti_launch(vec ? beam_merge_kernel<true> : beam_merge_kernel<false>, dim3(groups), dim3(MT), 0, stream, m));
     return 0;
 }

@@ -266,8 +266,9 @@ class BeamStepper:
         from ..kernels import beam as KB
         with self.engine.tracer.range("beam"):
             if scores is None:
-                scores = torch.zeros(self._slots.shape[0], 1, dtype=torch.float32, device=self.engine.device)
-            choice = KB.select(logits, scores, self.beams, self.stops)
+                # (64 bits: a score is a sum over all steps, and 32 would round the whole of it at each)
+                scores = torch.zeros(self._slots.shape[0], 1, dtype=torch.float64, device=self.engine.device)
+            choice = KB.select(logits, scores, self.beams, self.stops, **({"wide": True} if logits.is_cuda else {}))
             seen = None
             if logits.is_cuda:
                 seen = torch.cuda.Event()
@@ -311,12 +312,12 @@ class BeamStepper:
             n = wanted[0].numel()
             if self._side is None:
                 self._side = torch.cuda.Stream(device=choice.scores.device)
-            if self._host is None or self._host.shape[1] < n:
-                self._host = torch.empty((len(wanted), n), dtype=torch.int32, pin_memory=True)
+            if self._host is None or self._host[0].numel() < n:
+                self._host = [torch.empty(n, dtype=t.dtype, pin_memory=True) for t in wanted]
             with torch.cuda.stream(self._side):
                 self._side.wait_event(seen)
                 for row, t in zip(self._host, wanted):
-                    row[:n].copy_(t.reshape(-1).view(torch.int32), non_blocking=True)
+                    row[:n].copy_(t.view(n), non_blocking=True)
             self._side.synchronize()
-            host = [(row[:n] if t.dtype == torch.int32 else row[:n].view(torch.float32)).view(t.shape).tolist() for row, t in zip(self._host, wanted)]
+            host = [row[:n].view(t.shape).tolist() for row, t in zip(self._host, wanted)]
         return list(zip(*host))

@@ -21,7 +21,7 @@ from .wide import _fn
 from ..cache.allocators import PAGE
 
 P, I, L = c_void_p, c_int, c_longlong
-_SELECT = [P, L, I, I, I, P, I, P, I, I, P, P, P, P]
+_SELECT = [P, L, I, I, I, P, I, I, P, I, I, P, P, P, P]
 _TABLES = [P, I, P, P, P, I, I, I, I, I, P, P]
 _REORDER = [P, I, I, P, P, P, I, P]
 BEAMS_MAX = 32          # beams of one group
@@ -55,7 +55,8 @@ class Choice(NamedTuple):
     ended_tokens: torch.Tensor
 
 
-def select(logits: torch.Tensor, scores: torch.Tensor, beams: int, stop_ids: Optional[torch.Tensor] = None, ending: bool = True) -> Choice:
+def select(logits: torch.Tensor, scores: torch.Tensor, beams: int, stop_ids: Optional[torch.Tensor] = None, ending: bool = True,
+           wide: bool = False) -> Choice:
     """The next ``beams`` beams of every group.  logits float32 [groups * held, vocab] (a group's rows follow one another), scores
     float32 [groups, held] with held <= beams: the logarithms of the beams' probabilities so far (-inf: no beam; its row is not read).
 
@@ -63,12 +64,14 @@ def select(logits: torch.Tensor, scores: torch.Tensor, beams: int, stop_ids: Opt
     first ``beams`` whose token is not in ``stop_ids`` (int32, at most 16) are the next beams; with ``ending`` those among the first
     ``beams`` of all whose token is in it are returned as ended.  NaN counts as -inf, +inf as the largest finite number, and what is
     at -inf is never chosen: a group with fewer continuations keeps places without a beam.  The first child of a beam stays at its
-    place, the other children take the places of beams without one, in order.  Totals are formed in 64 bits and returned in 32."""
+    place, the other children take the places of beams without one, in order.  Totals are formed in 64 bits and returned in 32.  With ``wide`` scores are float64, those
+    given and those returned: for searches that hand them on from step to step, where each rounding to 32 bits would be one of the
+    whole sum."""
     _here(logits, scores, stop_ids, what="beam select")
     if logits.dtype != torch.float32 or logits.dim() != 2 or logits.stride(1) != 1:
         raise KernelError("beam select: expected float32 [rows, vocab] with dense rows")
-    if scores.dtype != torch.float32 or scores.dim() != 2 or not scores.is_contiguous():
-        raise KernelError("beam select: scores must be dense float32 [groups, beams]")
+    if scores.dtype != (torch.float64 if wide else torch.float32) or scores.dim() != 2 or not scores.is_contiguous():
+        raise KernelError(f"beam select: scores must be dense {'float64' if wide else 'float32'} [groups, beams]")
     G, held = scores.shape
     R, V = logits.shape
     if R != G * held or R == 0 or V == 0:
@@ -84,12 +87,17 @@ def select(logits: torch.Tensor, scores: torch.Tensor, beams: int, stop_ids: Opt
             raise KernelError(f"beam select: {n_stops} stop tokens (at most {STOPS_MAX})")
     # results and scratch in one piece: each allocation takes the host as long as half a launch
     n = G * beams
-    at = (6 * n + 3) & ~3
+    words = 4 * n if wide else 2 * n              # of the scores
+    at = (words + 4 * n + 3) & ~3
     room = torch.empty(at + R * (-(-V // TILE)) * PART, dtype=torch.int32, device=logits.device)
     base = room.data_ptr()
     _call(_fn("ti_beam_select", _SELECT),
-          logits.data_ptr(), logits.stride(0) if R > 1 else V, G, held, V, scores.data_ptr(), beams, _ptr(stop_ids), n_stops, 1 if ending else 0,
-          base, base + 8 * n, base + 4 * at, _stream(), launches=2)
+          logits.data_ptr(), logits.stride(0) if R > 1 else V, G, held, V, scores.data_ptr(), 1 if wide else 0, beams, _ptr(stop_ids), n_stops,
+          1 if ending else 0, base, base + 4 * words, base + 4 * at, _stream(), launches=2)
+    if wide:
+        scores, ended_scores = room[:words].view(torch.float64).view(2, G, beams).unbind(0)
+        parents, tokens, ended_parents, ended_tokens = room.as_strided((4, G, beams), (n, beams, 1), words).unbind(0)
+        return Choice(scores, parents, tokens, ended_scores, ended_parents, ended_tokens)
     scores, ended_scores, parents, tokens, ended_parents, ended_tokens = room.as_strided((6, G, beams), (n, beams, 1)).unbind(0)
     return Choice(scores.view(torch.float32), parents, tokens, ended_scores.view(torch.float32), ended_parents, ended_tokens)
 
