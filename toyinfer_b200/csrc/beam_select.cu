@@ -18,7 +18,7 @@
 //
 // Totals, sums and the order are in 64 bits, a sum good to 5e-11: beams compete by sums over a whole vocabulary, and at 32 bits the
 // order of two candidates of different rows would depend on how the sums were split.  Scores come and go in 32 or in 64 bits: a search
-// that hands them over in 32 rounds the whole sum at every step, 3e-2 after 8,000 tokens.
+// that hands them over in 32 rounds the whole sum at every step, and after 1,500 tokens near -3.7 each was off by 0.016.
 #include "common.cuh"
 
 namespace {
@@ -82,25 +82,11 @@ struct __align__(16) Part {              // of a tile
     float ref;           // 0, or ``top`` where the exponentials would leave the range of 64 bits
 };
 
-// Scores are float32 or float64, as the caller has them.
-struct Scores {
-    const void* at;
-    int wide;
-};
-__device__ __forceinline__ double score_at(Scores s, size_t i) {
-    const void* p = ti_dependent(s.at);
-    return s.wide ? static_cast<const double*>(p)[i] : (double)static_cast<const float*>(p)[i];
-}
-__device__ __forceinline__ void put_score(void* out, int wide, size_t i, double score) {
-    if (wide) static_cast<double*>(out)[i] = score;
-    else static_cast<float*>(out)[i] = (float)score;
-}
-
 struct ScanArgs {
     const float* logits;
     long long ld;
     int V, tiles;
-    Scores scores;
+    const void* scores;  // float32 or float64: the kernels' S
     Part* part;          // [rows, tiles]
 };
 
@@ -128,7 +114,7 @@ __device__ __forceinline__ void load_tile(float (&v)[LANE], const float* x, int 
 }
 
 // A lane's entries, and so the order of a row's sum, depend on their places alone: equal rows have equal sums.
-template <bool VEC>
+template <bool VEC, typename S>
 __global__ void __launch_bounds__(SCAN_WARPS * 32, 16) beam_scan_kernel(ScanArgs a) {
     ti_pdl_trigger();
     __shared__ double table[16];
@@ -137,8 +123,9 @@ __global__ void __launch_bounds__(SCAN_WARPS * 32, 16) beam_scan_kernel(ScanArgs
         table[threadIdx.x] = __hiloint2double(__double2hiint(pow16[threadIdx.x]) - ((int)threadIdx.x << 16), __double2loint(pow16[threadIdx.x]));
     __syncthreads();
     ti_pdl_sync();
+    const S* scores = static_cast<const S*>(ti_dependent(a.scores));
     const float* x = ti_dependent(a.logits) + (size_t)row * a.ld;
-    if (tile >= a.tiles || !(score_at(a.scores, row) > -INFINITY)) return;      // (the merge leaves such a row out as well)
+    if (tile >= a.tiles || !(scores[row] > (S)-INFINITY)) return;      // (the merge leaves such a row out as well)
     float v[LANE];
     load_tile<VEC>(v, x, tile * TILE, a.V, lane);
     float top = -INFINITY;
@@ -199,7 +186,7 @@ __device__ __forceinline__ unsigned bound_of(const unsigned* __restrict__ keys, 
 struct MergeArgs {
     const float* logits;
     long long ld;
-    Scores scores;           // [groups, held]
+    const void* scores;      // [groups, held]
     const Part* part;
     const int* stops;
     int held, beams, n_stops, tiles, V, ending;
@@ -214,7 +201,7 @@ struct MergeArgs {
 // What a block of the merge spends is latency: instructions that a block runs once come from L2 as its data do, so the code is kept
 // in loops, and what is rare is out of the way.  Behind the scan it takes 5 us for one row of 151,936 as for a group of four, 10
 // for 24 rows of 123,373 at odd addresses (12 with 512 threads, 19 with 256; one row 0.5 us less with 512).
-template <bool VEC>
+template <bool VEC, typename S>
 __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
     ti_pdl_trigger();
     __shared__ unsigned tile_key[KEYS];                              // a tile's top logit, then its largest total's key
@@ -224,7 +211,7 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
     __shared__ int tile_list[TILES];                                 // beam << 24 | tile
     __shared__ double row_add[BEAMS_MAX], row_ref[BEAMS_MAX];        // a total is row_add + (x - row_ref); row_add -infinity: no beam
     __shared__ float row_cut[BEAMS_MAX];                             // logits below it do not reach the bound
-    __shared__ double next_score[BEAMS_MAX];
+    __shared__ S next_score[BEAMS_MAX];
     __shared__ int next_parent[BEAMS_MAX], next_token[BEAMS_MAX], free_place[BEAMS_MAX];
     __shared__ int stops[STOPS_MAX];
     __shared__ int n_tiles, n_found, s_first;
@@ -240,13 +227,15 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
     }
     if (tid == 0) n_tiles = n_found = 0;
     ti_pdl_sync();
+    const S* scores = static_cast<const S*>(ti_dependent(a.scores)) + (size_t)g * a.held;
+    S *out_score = static_cast<S*>(a.out_score), *end_score = static_cast<S*>(a.end_score);
     const float* logits = ti_dependent(a.logits) + (size_t)g * a.held * a.ld;
     const Part* part = ti_dependent(a.part) + (size_t)g * all;
     const int* stop_ids = ti_dependent(a.stops);
     const size_t o = (size_t)g * a.beams;
     if (tid < a.n_stops) stops[tid] = stop_ids[tid];
     if (tid < a.beams) {
-        put_score(a.end_score, a.scores.wide, o + tid, -INFINITY);
+        end_score[o + tid] = (S)-INFINITY;
         a.end_parent[o + tid] = -1;
         a.end_token[o + tid] = -1;
     }
@@ -269,7 +258,7 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
 #pragma unroll 1
     for (int b = warp; b < a.held; b += MW) {
         const Part* p = part + (size_t)b * a.tiles;
-        const double score = score_at(a.scores, (size_t)g * a.held + b);
+        const S score = scores[b];
         bool some = false, shifted = false;
         double sum = 0.0;
         Part q[HELD];
@@ -285,7 +274,7 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
                     sum += q[j].sum;
                 }
         }
-        const bool there = score > -INFINITY && __any_sync(0xffffffffu, some);      // (nothing was written for a row without a beam)
+        const bool there = score > (S)-INFINITY && __any_sync(0xffffffffu, some);      // (nothing was written for a row without a beam)
         float m = 0.f;
         if (there && __any_sync(0xffffffffu, shifted)) {
             // tiles that were taken against another reference than 0: all against the largest of them
@@ -301,7 +290,7 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
         }
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        const double add = there ? score - log(sum) : -INFINITY, ref = m;
+        const double add = there ? (double)score - log(sum) : -INFINITY, ref = m;
         if (lane == 0) {
             row_add[b] = add;
             row_ref[b] = ref;
@@ -439,7 +428,7 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
     }
     // what has rank ``rank`` among all and ``open`` among those that are no stop tokens (whose: beam, token and the stop bit)
     auto settle = [&](unsigned long long key, unsigned long long whose, int rank, int open) {
-        const double total = total_of(key);
+        const S total = (S)total_of(key);
         if (whose < STOP) {
             if (open < a.beams) {
                 next_score[open] = total;
@@ -447,7 +436,7 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
                 next_token[open] = (int)whose;
             }
         } else if (a.ending && rank < a.beams) {
-            put_score(a.end_score, a.scores.wide, o + rank, total);
+            end_score[o + rank] = total;
             a.end_parent[o + rank] = (int)((whose & ~STOP) >> 32);
             a.end_token[o + rank] = (int)whose;
         }
@@ -593,12 +582,12 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
     const int place = stays ? p : there ? free_place[__popc(goes & below)] : -1;
     const unsigned taken = __reduce_or_sync(0xffffffffu, place >= 0 ? 1u << place : 0u);
     if (place >= 0) {
-        put_score(a.out_score, a.scores.wide, o + place, next_score[lane]);
+        out_score[o + place] = next_score[lane];
         a.out_parent[o + place] = p;
         a.out_token[o + place] = next_token[lane];
     }
     if (lane < a.beams && !((taken >> lane) & 1u)) {
-        put_score(a.out_score, a.scores.wide, o + lane, -INFINITY);
+        out_score[o + lane] = (S)-INFINITY;
         a.out_parent[o + lane] = lane;
         a.out_token[o + lane] = 0;
     }
@@ -620,14 +609,17 @@ extern "C" int ti_beam_select(const float* logits, long long ld, int groups, int
     const int tiles = (V + TILE - 1) / TILE;
     TI_REQUIRE(tiles < 1 << 24, "beam select: %d logits a row", V);
     const bool vec = ld % 4 == 0 && (reinterpret_cast<uintptr_t>(logits) & 15) == 0;
-    const Scores from = {scores, wide_scores};
-    ScanArgs s = {logits, ld, V, tiles, from, static_cast<Part*>(scratch)};
+    ScanArgs s = {logits, ld, V, tiles, scores, static_cast<Part*>(scratch)};
     const dim3 grid((tiles + SCAN_WARPS - 1) / SCAN_WARPS, (unsigned)rows);
-    TI_CUDA(ti_launch(vec ? beam_scan_kernel<true> : beam_scan_kernel<false>, grid, dim3(SCAN_WARPS * 32), 0, stream, s));
+    auto scan = wide_scores ? (vec ? beam_scan_kernel<true, double> : beam_scan_kernel<false, double>)
+                            : (vec ? beam_scan_kernel<true, float> : beam_scan_kernel<false, float>);
+    TI_CUDA(ti_launch(scan, grid, dim3(SCAN_WARPS * 32), 0, stream, s));
     const size_t n = (size_t)groups * beams;
     void* ended = static_cast<char*>(out_scores) + n * (wide_scores ? 8 : 4);
-    MergeArgs m = {logits, ld, from, s.part, stops, held, beams, n_stops, tiles, V, ending,
+    MergeArgs m = {logits, ld, scores, s.part, stops, held, beams, n_stops, tiles, V, ending,
                    out_scores, out_places, out_places + n, ended, out_places + 2 * n, out_places + 3 * n};
-    TI_CUDA(ti_launch(vec ? beam_merge_kernel<true> : beam_merge_kernel<false>, dim3(groups), dim3(MT), 0, stream, m));
+    auto merge = wide_scores ? (vec ? beam_merge_kernel<true, double> : beam_merge_kernel<false, double>)
+                             : (vec ? beam_merge_kernel<true, float> : beam_merge_kernel<false, float>);
+    TI_CUDA(ti_launch(merge, dim3(groups), dim3(MT), 0, stream, m));
     return 0;
 }
