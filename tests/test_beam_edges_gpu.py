@@ -88,3 +88,58 @@ def test_select_refuses_scores_of_other_types():
                  (wide[:, :2].contiguous().half(), True)):
         with pytest.raises(KernelError, match="scores"):
             KB.select(x, s, 2, wide=w)
+
+
+def groups_with_homes(G, B, width, length, seed):
+    """Slots, homes (a page of its own per place and column), tables as a search leaves them, and parents with places that move."""
+    rng = np.random.RandomState(seed)
+    slots = rng.permutation(G * B + 1)[:G * B].reshape(G, B).astype(np.int32)
+    home = np.zeros((G * B + 2, width), dtype=np.int32)
+    home[:-1] = 1 + rng.permutation((G * B + 1) * width).reshape(-1, width)
+    table = home.copy()
+    for g in range(G):
+        for c in range(width):
+            pick = rng.permutation(B) if c == length // 64 else rng.randint(0, B, B)
+            table[slots[g], c] = home[slots[g][pick], c]
+    parents = np.tile(np.arange(B, dtype=np.int32), (G, 1))
+    parents[:, 1:B:2] = 0
+    return slots, home, table, parents
+
+
+@pytest.mark.parametrize("B,n_tables,which,fault", [(4, 1, 0, "none"), (4, 1, 0, "twice"), (3, 2, 1, "none"), (32, 2, 0, "twice"), (5, 8, 6, "none"),
+                                                    (2, 5, 4, "negative")])
+def test_a_group_without_a_page_per_beam_is_left_as_it_was(B, n_tables, which, fault):
+    """One of three groups lacks a page of its own at the column that is written, in one table of several: the group is reported, and nothing
+    of it changes or moves in any table; the other two groups go on."""
+    from toyinfer_b200 import kernels as K
+    from toyinfer_b200.kernels import beam as KB
+    length, width = 150, 4
+    made = [groups_with_homes(3, B, width, length, 7) for _ in range(n_tables)]
+    slots, _, _, parents = made[0]
+    homes, tables = [m[1].copy() for m in made], [m[2].copy() for m in made]
+    homes[which][slots[1, B - 1], length // 64] = {"none": 0, "negative": -3, "twice": homes[which][slots[1, 0], length // 64]}[fault]
+    dev = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(DEV)       # noqa: E731
+    on_gpu = [dev(t) for t in tables]
+    moves = KB.tables(dev(slots), dev(parents), dev(np.full(3, length, dtype=np.int32)), 0,
+                      [KB.Table(t, dev(h)) for t, h in zip(on_gpu, homes)])
+    with pytest.raises(K.KernelError, match="out of place"):
+        K.check_status()
+    rest = [0, 2]
+    want_tables = [t.copy() for t in tables]
+    want = plain.tables(want_tables, homes, [0] * n_tables, slots[rest], parents[rest], [length] * 2).reshape(1 + n_tables, 2, B, 3)
+    got = moves.cpu().numpy().reshape(1 + n_tables, 3, B, 3)
+    assert np.array_equal(got[:, rest], want) and not got[:, 1].any()
+    for t, w in zip(on_gpu, want_tables):
+        assert np.array_equal(t.cpu().numpy(), w)            # (the plain form has left the group's rows alone)
+
+
+def test_a_group_in_which_nothing_moves_needs_no_pages():
+    from toyinfer_b200 import kernels as K
+    from toyinfer_b200.kernels import beam as KB
+    slots, home, table, _ = groups_with_homes(2, 4, 3, 70, 3)
+    parents = np.tile(np.arange(4, dtype=np.int32), (2, 1))
+    dev = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(DEV)       # noqa: E731
+    t = dev(table)
+    moves = KB.tables(dev(slots), dev(parents), dev(np.full(2, 70, dtype=np.int32)), 0, [KB.Table(t, torch.zeros_like(t))])
+    K.check_status()
+    assert not moves.any().item() and np.array_equal(t.cpu().numpy(), table)

@@ -118,7 +118,8 @@ def tables(slots: torch.Tensor, parents: torch.Tensor, lengths: torch.Tensor, ex
     slots and parents int32 [groups, beams], parents as ``select`` gives them; lengths int32 [groups]: the positions that each
     group's sequences hold are lengths + extra.  A page that is not written any more is shared by the places that come from its
     beam; at the column that the next token goes to every place gets a page of its own, out of the group's homes there, and the
-    rows that it holds so far are among the moves.  At that column the homes of a group are pages of its own, one per place.
+    rows that it holds so far are among the moves.  At that column the homes of a group are pages of its own, one per place; a group
+    whose are not is reported (``check_status``) and left as it was, and so is a place whose parent or slot is out of place.
     ``reorder`` comes next, before anything reads the tables or writes the pages."""
     _here(slots, parents, lengths, what="beam tables")
     for t, what in ((slots, "slots"), (parents, "parents"), (lengths, "lengths")):
@@ -146,7 +147,7 @@ def tables(slots: torch.Tensor, parents: torch.Tensor, lengths: torch.Tensor, ex
     moves = torch.empty((1 + n_tables, G * B, 3), dtype=torch.int32, device=slots.device)
     _call(_fn("ti_beam_tables", _TABLES), (c_longlong * len(words))(*words), n_tables, slots.data_ptr(),
           parents.data_ptr(), lengths.data_ptr(), int(extra), G, B, PAGE, n_slots if n_slots is not None else 1 << 30, moves.data_ptr(),
-          _stream(), launches=max(1, -(-n_tables // 4)))
+          _stream())
     return moves
 
 
