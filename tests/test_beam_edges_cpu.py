@@ -1,7 +1,10 @@
 """Beam search's bookkeeping at its edges, without a device: scores over long searches, limits, options."""
 from __future__ import annotations
 
+import types
+
 import numpy as np
+import pytest
 import torch
 
 from beam_edges import LastTokenModel, best_chains
@@ -34,3 +37,31 @@ def test_scores_of_a_long_search_are_sums_in_64_bits(monkeypatch):
         assert abs(h.score - sum(lp[a, b] for a, b in zip(path, path[1:]))) <= 1e-8
         assert abs(h.score - score) <= 1e-8
         assert h.tokens == tokens[1:]
+
+
+@pytest.mark.parametrize("penalty", ["9", "-1", "nan", "0.5"])
+def test_without_beam_search_any_length_penalty_is_taken(monkeypatch, capsys, penalty):
+    import toyinfer_b200
+    from toyinfer_b200.engine import cli
+
+    class Fake:
+        engine = types.SimpleNamespace(spec=types.SimpleNamespace(vocab_size=10))
+        last_stats = types.SimpleNamespace(prompt_tokens=1, generated_tokens=2)
+
+        def __init__(self, *args, **kw):
+            pass
+
+        def generate(self, prompts, *args, **kw):
+            return [types.SimpleNamespace(tokens=[4, 5], finish_reason="length") for _ in prompts]
+
+    monkeypatch.setattr(toyinfer_b200, "LLM", Fake)
+    assert cli.main(["--model_dir", "x", "--prompt_ids", "1", "--length_penalty", penalty]) == 0
+    assert '"tokens": [4, 5]' in capsys.readouterr().out
+    if penalty != "0.5":
+        assert cli.main(["--model_dir", "x", "--prompt_ids", "1", "--length_penalty", penalty, "--beam_size", "2"]) == 2
+
+
+def test_a_folder_without_a_model_is_an_error_of_the_call(capsys):
+    from toyinfer_b200.engine import cli
+    assert cli.main(["--model_dir", "nowhere", "--prompt_ids", "1"]) == 2
+    assert "nowhere" in capsys.readouterr().err

@@ -65,7 +65,8 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--top_p", type=float, default=0.95)
     ap.add_argument("--beam_size", type=int, default=1, help="beams per request (1: no beam search); with more, the best "
                     "hypothesis is printed and the sampling options have no effect")
-    ap.add_argument("--length_penalty", type=float, default=1.0, help="beam search ranks hypotheses by score / tokens ** length_penalty")
+    ap.add_argument("--length_penalty", type=float, default=1.0, help="beam search ranks hypotheses by score / tokens ** length_penalty (0 to 5; "
+                    "no effect with --beam_size 1)")
     # beyond the reference
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
     ap.add_argument("--prompt_ids", default="", help='token ids: "1,2,3;4,5" or a file')
@@ -112,13 +113,14 @@ def main(argv=None) -> int:
     args = build_parser().parse_args(argv)
     from ..sampling import BeamParams
     beams = BeamParams(beams=args.beam_size, length_penalty=args.length_penalty)
-    try:
-        beams.check()
-        if args.beam_size > args.max_batch:
-            raise ValueError(f"--beam_size {args.beam_size} exceeds --max_batch {args.max_batch}")
-    except ValueError as exc:
-        print(f"toyinfer: {exc}", file=sys.stderr)
-        return 2
+    if args.beam_size != 1:              # (without beam search --length_penalty has no effect, whatever it is)
+        try:
+            beams.check()
+            if args.beam_size > args.max_batch:
+                raise ValueError(f"--beam_size {args.beam_size} exceeds --max_batch {args.max_batch}")
+        except ValueError as exc:
+            print(f"toyinfer: {exc}", file=sys.stderr)
+            return 2
     if bool(args.model_dir) == bool(args.random):
         print("toyinfer: give either --model_dir or --random CONFIG_JSON", file=sys.stderr)
         return 2
@@ -127,15 +129,20 @@ def main(argv=None) -> int:
         return 2
     import torch
     from .. import LLM, SamplingParams
+    from ..config.base import ConfigError
 
     common = dict(dtype=args.dtype, max_seq_len=args.max_seq_len or None, max_batch=args.max_batch,
                   enable_cuda_graph=args.enable_cuda_graph, use_dedicated_prefill=args.use_dedicated_prefill,
                   detail_time=args.detail_time, prefill_chunk=args.prefill_chunk or None)
-    if args.random:
-        with open(args.random) as f:
-            llm = LLM(config=json.load(f), seed=args.seed, **common)
-    else:
-        llm = LLM(args.model_dir, **common)
+    try:
+        if args.random:
+            with open(args.random) as f:
+                llm = LLM(config=json.load(f), seed=args.seed, **common)
+        else:
+            llm = LLM(args.model_dir, **common)
+    except ConfigError as exc:           # no folder, or a config.json that cannot be used
+        print(f"toyinfer: {exc}", file=sys.stderr)
+        return 2
     vocab = llm.engine.spec.vocab_size
     max_new = args.max_new_tokens
     ignore_eos = args.ignore_eos
