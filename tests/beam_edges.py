@@ -13,7 +13,7 @@ class LastTokenModel:
     def __init__(self, logits):
         self.logits, self.device, self.slots = logits, logits.device, 0
         self.tracer = types.SimpleNamespace(range=lambda name: contextlib.nullcontext())
-        self.cache = types.SimpleNamespace(beam_tokens=lambda prompt, length, beams: 64, reserve_beams=lambda *a: None,
+        self.cache = types.SimpleNamespace(beam_groups=lambda beams: 64, beam_tokens=lambda prompt, length, beams: 64, reserve_beams=lambda *a: None,
                                            begin_beams=lambda *a: None, follow_parents=lambda *a: None, kv_groups=[])
 
     def new_sequence(self):

@@ -7,10 +7,15 @@ import numpy as np
 import pytest
 import torch
 
+import cpu_beam
+import cpu_kernels
 from beam_edges import LastTokenModel, best_chains
+from conftest import prompts_for
 from plain import beam_plain
-from toyinfer_b200 import BeamParams
-from toyinfer_b200.engine.beam import BeamLoop, BeamStepper
+from toyinfer_b200 import LLM, BeamParams
+from toyinfer_b200.cache import CacheError
+from toyinfer_b200.engine.beam import BeamLoop, BeamStepper, plan_beams
+from toyinfer_b200.kernels import KernelError
 from toyinfer_b200.kernels import beam as KB
 
 
@@ -65,3 +70,58 @@ def test_a_folder_without_a_model_is_an_error_of_the_call(capsys):
     from toyinfer_b200.engine import cli
     assert cli.main(["--model_dir", "nowhere", "--prompt_ids", "1"]) == 2
     assert "nowhere" in capsys.readouterr().err
+
+
+@pytest.fixture()
+def cpu_llm(monkeypatch, model_folders):
+    cpu_kernels.install(monkeypatch)
+    cpu_beam.install(monkeypatch)
+    return lambda name, **kw: LLM(model_folders[name], dtype="float32", device="cpu", **{"max_batch": 8, "max_tokens": 2048, **kw})
+
+
+def test_a_batch_holds_no_more_groups_than_one_move_takes(cpu_llm, monkeypatch):
+    """The move takes so many entries over all lists (states and page tables): more requests run in further batches."""
+    llm = cpu_llm("A", max_seq_len=64, max_batch=8)
+    lists = 1 + len(llm.engine.cache.kv_groups)
+    prompts = prompts_for("A", [5, 6, 7, 8, 9], seed=2)
+    want = llm.beam_search(prompts, BeamParams(2, n_best=2), max_new_tokens=4, ignore_eos=True)
+    assert llm.last_stats.batches == 2
+    monkeypatch.setattr(KB, "MOVES_MAX", lists * 5)          # two groups of two beams, not three
+    tables = KB.tables
+
+    def limited(slots, *args):
+        assert slots.numel() * lists <= KB.MOVES_MAX
+        return tables(slots, *args)
+
+    monkeypatch.setattr(KB, "tables", limited)
+    got = llm.beam_search(prompts, BeamParams(2, n_best=2), max_new_tokens=4, ignore_eos=True)
+    assert llm.last_stats.batches == 3
+    assert [[h.tokens for h in g] for g in got] == [[h.tokens for h in g] for g in want]
+
+
+def test_a_cache_that_cannot_hold_beams_is_refused_before_anything_runs(cpu_llm, monkeypatch):
+    """More page tables than one call takes, or memory that cannot be moved."""
+    llm = cpu_llm("C", max_seq_len=64)                        # full and windowed layers: two tables
+    c = llm.engine.cache
+    assert len(c.kv_groups) == 2
+    monkeypatch.setattr(llm.engine, "step", lambda *a, **k: pytest.fail("a step ran"))
+    monkeypatch.setattr(KB, "TABLES_MAX", 1)
+    with pytest.raises(CacheError, match="page tables"):
+        llm.beam_search([[1, 2]], BeamParams(2), ignore_eos=True)
+    monkeypatch.setattr(KB, "TABLES_MAX", 8)
+
+    def refusing(states, pages):
+        raise KernelError("cannot be moved")
+
+    monkeypatch.setattr(KB, "Areas", refusing)
+    c._areas = None
+    with pytest.raises(KernelError, match="cannot be moved"):
+        llm.beam_search([[1, 2]], BeamParams(2), ignore_eos=True)
+    assert c.slots.n_free == c.n_slots
+
+
+def test_plan_by_positions():
+    """A request that fills the cache to the last position shares a batch; one position less, and it does not."""
+    assert plan_beams([64, 640, 64], 8, 704) == [[0, 1], [2]]
+    assert plan_beams([64, 640, 64], 8, 703) == [[0], [1], [2]]
+    assert plan_beams([64, 640, 64], 8, 768) == [[0, 1, 2]]

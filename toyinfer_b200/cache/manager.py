@@ -235,6 +235,20 @@ class CacheManager:
             g.grow(slot, new_length)
 
     # -- beams ------------------------------------------------------------------
+    def _beam_areas(self):
+        from ..kernels import beam as KB
+        if self._areas is None:
+            self._areas = KB.Areas(list(self.states.values()), [[g.k] if g.v is None else [g.k, g.v] for g in self.kv_groups])
+        return self._areas
+
+    def beam_groups(self, beams: int) -> int:
+        """Groups of ``beams`` that ``follow_parents`` takes at a time; raises where the cache cannot hold beams at all."""
+        from ..kernels import beam as KB
+        if len(self.kv_groups) > KB.TABLES_MAX:
+            raise CacheError(f"beams over {len(self.kv_groups)} page tables (at most {KB.TABLES_MAX})")
+        self._beam_areas()
+        return min(KB.MOVES_MAX // (1 + len(self.kv_groups)), KB.ROWS_MAX) // beams
+
     def beam_tokens(self, prompt: int, length: int, beams: int) -> int:
         """Positions, in whole pages, that a request's beams may come to hold: the most of any group."""
         most = 0
@@ -267,10 +281,8 @@ class CacheManager:
         """Lets every place of the groups ``slots`` [groups, beams] go on from the place ``parents`` names (kernels/beam.py:
         tables, reorder); the sequences hold ``lengths`` [groups] + extra positions.  All on the device, in the stream's order."""
         from ..kernels import beam as KB
-        if self._areas is None:
-            self._areas = KB.Areas(list(self.states.values()), [[g.k] if g.v is None else [g.k, g.v] for g in self.kv_groups])
         moves = KB.tables(slots, parents, lengths, extra, [KB.Table(g.table, g.home, g.ring_rows) for g in self.kv_groups])
-        KB.reorder(self._areas, moves)
+        KB.reorder(self._beam_areas(), moves)
 
     def commit(self, slot: int, new_length: int) -> None:
         self.length[slot] = new_length

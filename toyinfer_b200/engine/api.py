@@ -161,7 +161,8 @@ class LLM:
     def beam_search(self, prompts: Sequence[Sequence[int]], beams: Optional[BeamParams] = None, max_new_tokens: int = 16,
                     stop_token_ids: Optional[Sequence[int]] = None, ignore_eos: bool = False) -> List[List[Hypothesis]]:
         """The ``beams.n_best`` best hypotheses of every prompt, best first.  Each request takes ``beams.beams`` of the engine's
-        ``max_batch`` places; the beams share the pages of their prompt."""
+        ``max_batch`` places; the beams share the pages of their prompt.  At most 16 stop tokens, the model's own among them
+        (``generate`` takes any number), and a cache of at most eight page tables."""
         beams = beams or BeamParams()
         beams.check()
         stops = set()

@@ -10,8 +10,8 @@ A hypothesis ends at a stop token that is among the ``beams`` best continuations
 its tokens, but of its score and of the count that its value divides by), after ``max_new_tokens``, or when it holds
 ``max_seq_len`` positions.
 
-The loop only decides.  It runs steps through a ``stepper`` with ``open(prompt, length) -> slots``, ``close(slots)``,
-``tokens_needed(prompt, length)``, ``prompt(entries, want) -> logits``, ``stack(rows) -> logits``, ``begin(groups)``,
+The loop only decides.  It runs steps through a ``stepper`` with ``groups_at_once``, ``open(prompt, length) -> slots``,
+``close(slots)``, ``tokens_needed(prompt, length)``, ``prompt(entries, want) -> logits``, ``stack(rows) -> logits``, ``begin(groups)``,
 ``select(logits, scores, drawn) -> choice``, ``step(slots, choice, groups) -> logits``, ``read(choice)``, ``keep(logits,
 groups)`` and ``carry(choice, groups) -> scores``, so that its decisions can be tested without a device.
 
@@ -137,7 +137,7 @@ class BeamLoop:
             else:
                 todo.append(i)
         needs = [self.stepper.tokens_needed(len(prompts[i]), min(len(prompts[i]) + max_new, self.max_seq_len)) for i in todo]
-        for batch in plan_beams(needs, self.max_batch // self.params.beams, self.capacity_tokens):
+        for batch in plan_beams(needs, min(self.max_batch // self.params.beams, self.stepper.groups_at_once), self.capacity_tokens):
             self._run_batch([todo[k] for k in batch], prompts, max_new, results)
         return results
 
@@ -222,6 +222,8 @@ class BeamStepper:
         if len(stop_ids) > KB.STOPS_MAX:
             raise ValueError(f"{len(stop_ids)} stop tokens (beam search takes {KB.STOPS_MAX})")
         self.engine, self.beams = engine, params.beams
+        # what a cache may not have is found here, not after the prompts have run
+        self.groups_at_once = engine.cache.beam_groups(params.beams)
         self.stops = torch.tensor(sorted(stop_ids), dtype=torch.int32, device=engine.device) if len(stop_ids) else None
         self._side = self._host = None
         self._slots = self._lengths = None

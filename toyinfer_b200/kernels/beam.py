@@ -27,6 +27,7 @@ _REORDER = [P, I, I, P, P, P, I, P]
 BEAMS_MAX = 32          # beams of one group
 STOPS_MAX = 16          # stop tokens
 TABLES_MAX = 8          # page tables of one cache
+ROWS_MAX = 65535        # rows of logits of one selection
 MOVES_MAX = 8192        # entries of one call's moves, over its lists
 TILE, PART = 1024, 4    # logits of a row that csrc/beam_select.cu takes at a time, and the words of scratch for them
 PIECE = 16384           # bytes that a warp moves at a time (csrc/beam_reorder.cu)
