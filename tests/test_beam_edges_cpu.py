@@ -125,3 +125,19 @@ def test_plan_by_positions():
     assert plan_beams([64, 640, 64], 8, 704) == [[0, 1], [2]]
     assert plan_beams([64, 640, 64], 8, 703) == [[0], [1], [2]]
     assert plan_beams([64, 640, 64], 8, 768) == [[0, 1, 2]]
+
+
+def test_sizes_that_pass_32_bits_are_refused(monkeypatch):
+    """Sizes go to the kernels as 32-bit numbers: 2^32 + 5 logits must not be taken as 5, nor 2^32 positions as none."""
+    monkeypatch.setattr(KB, "_here", lambda *tensors, what: None)
+    monkeypatch.setattr(KB, "_call", lambda *a, **k: pytest.fail("a kernel was launched"))
+    monkeypatch.setattr(KB, "_fn", lambda *a: None)
+    for V in ((1 << 32) + 5, (1 << 31) - 1, (1 << 30) + 1):
+        with pytest.raises(KernelError, match="logits"):
+            KB.select(torch.empty(2, V, device="meta"), torch.empty(1, 2, device="meta"), 2)
+    with pytest.raises(KernelError, match="rows"):
+        KB.select(torch.empty(65536, 8, device="meta"), torch.empty(32768, 2, device="meta"), 2)
+    slots = torch.zeros(1, 2, dtype=torch.int32)
+    for extra in (1 << 32, (1 << 31) - 1, -(1 << 31)):
+        with pytest.raises(KernelError, match="positions"):
+            KB.tables(slots, slots, slots[0, :1], extra, [])

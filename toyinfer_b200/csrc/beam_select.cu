@@ -599,7 +599,7 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
 extern "C" int ti_beam_select(const float* logits, long long ld, int groups, int held, int V, const void* scores, int wide_scores,
                               int beams, const int* stops, int n_stops, int ending, void* out_scores, int* out_places, void* scratch,
                               cudaStream_t stream) {
-    TI_REQUIRE(groups >= 1 && held >= 1 && V >= 1 && ld >= V, "beam select: %d groups of %d rows of %d logits, %lld apart", groups, held, V, ld);
+    TI_REQUIRE(groups >= 1 && held >= 1 && V >= 1 && V <= 1 << 30 && ld >= V, "beam select: %d groups of %d rows of %d logits, %lld apart", groups, held, V, ld);
     TI_REQUIRE(beams >= 1 && beams <= BEAMS_MAX && held <= beams, "beam select: %d beams from %d (at most %d, and no fewer than before)",
                beams, held, BEAMS_MAX);
     TI_REQUIRE(n_stops >= 0 && n_stops <= STOPS_MAX && (n_stops == 0 || stops), "beam select: %d stop tokens (at most %d)", n_stops, STOPS_MAX);
@@ -607,7 +607,6 @@ extern "C" int ti_beam_select(const float* logits, long long ld, int groups, int
     TI_REQUIRE(rows <= 65535, "beam select: %lld rows in one call (at most 65535)", rows);
     TI_REQUIRE(scratch != nullptr && (reinterpret_cast<uintptr_t>(scratch) & 15) == 0, "beam select: the scratch must start at 16 bytes");
     const int tiles = (V + TILE - 1) / TILE;
-    TI_REQUIRE(tiles < 1 << 24, "beam select: %d logits a row", V);
     const bool vec = ld % 4 == 0 && (reinterpret_cast<uintptr_t>(logits) & 15) == 0;
     ScanArgs s = {logits, ld, V, tiles, scores, static_cast<Part*>(scratch)};
     const dim3 grid((tiles + SCAN_WARPS - 1) / SCAN_WARPS, (unsigned)rows);

@@ -28,6 +28,7 @@ BEAMS_MAX = 32          # beams of one group
 STOPS_MAX = 16          # stop tokens
 TABLES_MAX = 8          # page tables of one cache
 ROWS_MAX = 65535        # rows of logits of one selection
+VOCAB_MAX = 1 << 30     # logits of a row: places inside a row are 32-bit numbers
 MOVES_MAX = 8192        # entries of one call's moves, over its lists
 TILE, PART = 1024, 4    # logits of a row that csrc/beam_select.cu takes at a time, and the words of scratch for them
 PIECE = 16384           # bytes that a warp moves at a time (csrc/beam_reorder.cu)
@@ -77,6 +78,8 @@ def select(logits: torch.Tensor, scores: torch.Tensor, beams: int, stop_ids: Opt
     R, V = logits.shape
     if R != G * held or R == 0 or V == 0:
         raise KernelError(f"beam select: {R} rows of {V} logits do not fit {G} groups of {held} beams")
+    if V > VOCAB_MAX or R > ROWS_MAX:
+        raise KernelError(f"beam select: {R} rows of {V} logits (at most {ROWS_MAX} of {VOCAB_MAX})")
     if not 1 <= held <= beams <= BEAMS_MAX:
         raise KernelError(f"beam select: {beams} beams from {held} (at most {BEAMS_MAX}, and no fewer than before)")
     n_stops = 0
@@ -133,6 +136,8 @@ def tables(slots: torch.Tensor, parents: torch.Tensor, lengths: torch.Tensor, ex
     n_tables = len(page_tables)
     if B > BEAMS_MAX or n_tables > TABLES_MAX:
         raise KernelError(f"beam tables: {B} beams, {n_tables} tables (at most {BEAMS_MAX} and {TABLES_MAX})")
+    if not -(1 << 30) <= extra <= 1 << 30:
+        raise KernelError(f"beam tables: {extra} positions behind the lengths")
     words = []
     n_slots = None
     for table, home, ring_rows in page_tables:
