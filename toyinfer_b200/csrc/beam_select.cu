@@ -32,9 +32,13 @@ constexpr int MW = MT / 32;
 constexpr int SIDES = MT / 256;      // tiles that are read again side by side
 constexpr int TILES = 512;           // tiles of a group that may reach the bound
 constexpr int ROOM = 1536;           // candidates above it; more than a tile and all that is kept of the ones before
-constexpr int KEYS = 3840;           // tiles of a group whose totals are kept in shared memory
+// Tiles of a group whose totals are kept in shared memory: what its 48 KB leave, 25 rows of 151,936 logits.  The others' parts are read again
+// from L2: 16 us for 26 such rows, 17 to 18 for 32, wherever the best scores are.
+constexpr int KEYS = 3840;
 constexpr int AHEAD = 2;             // tiles that each side has on the way at a time
-constexpr int HELD = 5;              // tiles of a row, of 32 each, whose parts a warp has on the way at a time
+// Tiles of a row, of 32 each, whose parts a warp has on the way at a time; rows of up to 5 * 32 * 1,024 = 163,840 logits are read once (24 of
+// them 15.9 us, 17.1 for 24 of 164,000).
+constexpr int HELD = 5;
 constexpr float BIG = 3.402823466e38f;
 constexpr float PLAIN = 600.f;       // |largest logit| of a tile up to which its exponentials are summed as they are
 constexpr float LEAST = -690.f;      // what lies below counts as this: e^-690, next to nothing beside e^-600
@@ -307,7 +311,7 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
         }
     }
     __syncthreads();
-    // (Tiles behind the shared ones are read again each time, and count for the bound only where there are no stop tokens.)
+    // (Tiles behind the shared ones are read again each time, and count for the bound only where they hold no stop token at all.)
     auto key_behind = [&](int i) {
         const int b = i / a.tiles;
         const float top = part[i].top;
@@ -318,9 +322,13 @@ __global__ void __launch_bounds__(MT) beam_merge_kernel(MergeArgs a) {
 #pragma unroll 2
     for (int i = tid; i < shared; i += MT)
         if (!((stop_tile[i >> 5] >> (i & 31)) & 1u)) mine = max(mine, tile_key[i]);
-    if (a.n_stops == 0)
 #pragma unroll 1
-        for (int i = KEYS + tid; i < all; i += MT) mine = max(mine, key_behind(i));
+    for (int i = KEYS + tid; i < all; i += MT) {
+        bool stop = false;
+#pragma unroll 1
+        for (int s = 0; s < a.n_stops; ++s) stop |= stops[s] / TILE == i % a.tiles;
+        if (!stop) mine = max(mine, key_behind(i));
+    }
     keys[tid] = mine;
     __syncthreads();
     // the bound, and below which logit a row's entries cannot reach it: a little lower, for the roundings of the two forms
