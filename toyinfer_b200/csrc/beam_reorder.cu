@@ -11,8 +11,8 @@
 // in one numbering, so a few moves of a small cache spread over the SMs as many moves of a large one do.  Widths of 16, 4 or 2
 // bytes, as the area's addresses and strides allow; a warp has eight loads on the way before its first store.  Four blocks an SM, all
 // resident, and pieces as long as a head's page keep what DRAM reads and writes in long runs: 32 moves of part pages of 36 layers (261
-// MB read and written) take 43.4 us; 46.1 with pieces of 8 KB, 45.8 with five blocks, 48.5 with three, 73 with sixteen loads on the
-// way; 39.9 at the copy rate.  Twelve states of 38 MB that start at any 4 bytes (911 MB) take 152 us, 139 at the copy rate.
+// MB read and written) take 43.5 us; 46.1 with pieces of 8 KB, 45.8 with five blocks, 48.5 with three, 73 with sixteen loads on the
+// way; 39.9 at the copy rate.  Twelve states of 38 MB that start at any 4 bytes (911 MB) take 151.7 us, 139 at the copy rate.
 #include "tma.cuh"
 
 namespace {
