@@ -178,3 +178,21 @@ def test_wide_groups_whose_best_beams_are_the_last(G, B, V, stops):
 
     time(None)
     assert time(ids) < 5 * time(None)
+
+
+def test_selections_with_wide_scores_in_one_graph():
+    """Two steps captured together, the second from the first one's scores where they lie; replayed with other logits."""
+    from toyinfer_b200.kernels import beam as KB
+    G, B, V = 3, 4, 20001
+    make = lambda seed: torch.randn(2, G * B, V, generator=torch.Generator(device=DEV).manual_seed(seed), device=DEV) * 2.5      # noqa: E731
+    start = -3000 + torch.arange(G * B, device=DEV, dtype=torch.float64).view(G, B) * 1e-5
+    two = lambda x: KB.select(x[1], KB.select(x[0], start, B, wide=True).scores, B, wide=True)                                  # noqa: E731
+    x = make(1)
+    two(x)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = two(x)
+    for seed in (2, 3):
+        x.copy_(make(seed))
+        g.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, two(x.clone())))

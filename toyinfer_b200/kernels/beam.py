@@ -119,8 +119,8 @@ def tables(slots: torch.Tensor, parents: torch.Tensor, lengths: torch.Tensor, ex
     """Lets the page tables follow the beams, in place, and returns what has to move: int32 [1 + tables, groups * beams, 3] with
     (source, destination, rows) per place, rows 0 where nothing does.  List 0 is slots (for states), list 1 + i pages of table i.
 
-    slots and parents int32 [groups, beams], parents as ``select`` gives them; lengths int32 [groups]: the positions that each
-    group's sequences hold are lengths + extra.  A page that is not written any more is shared by the places that come from its
+    slots and parents int32 [groups, beams], each slot in one group, parents as ``select`` gives them; lengths int32 [groups]: the
+    positions that each group's sequences hold are lengths + extra.  A page that is not written any more is shared by the places that come from its
     beam; at the column that the next token goes to every place gets a page of its own, out of the group's homes there, and the
     rows that it holds so far are among the moves.  At that column the homes of a group are pages of its own, one per place; a group
     whose are not is reported (``check_status``) and left as it was, and so is a place whose parent or slot is out of place.
